@@ -190,6 +190,65 @@ int grinqh_gemm_or_gemv_noalloc(const void* x, int64_t M, int64_t K, int64_t ldx
                                 int max_bits, int group_size, const float thresholds[4], int mode,
                                 void* stream);
 
+/* ---- Attention between the quantized linears (no counterpart in the
+ * reference, which leaves attention to vLLM): a key/value cache held in 4 bits,
+ * filled, read back and attended to by one query token per sequence, and the
+ * attention over whole prompts.  head_dim is 64, 128 or 256; q, k and v rows are
+ * [token][head][head_dim] with the given element distances of tokens and heads
+ * (multiples of 8, at most 2^23; 16-byte aligned, channels adjacent), as slices
+ * of a fused projection are; results are dense.
+ *
+ * The cache is uint8 [pages][kv_heads][page_size / 16][record], page_size 16
+ * times a power of two, 64-byte aligned.  A record (grinqh_kv4_record_bytes)
+ * holds 16 tokens of one head: the keys' codes (words of 8 channels: word
+ * (c / 8) % 4 * (head_dim / 32) + c / 32 of a token), their (scale, minimum) fp16
+ * pairs [head_dim / group][16], the values' codes [head_dim / 8][16 tokens] and
+ * their pairs [16]; channel c of a word's 8 is nibble c / 2 + 4 (c % 2).  Keys have
+ * one pair per `group` channels (32, 64, 128 or 256, at most head_dim), values one per token and
+ * head.  Values are limited to +-65504; minimum = f16(min), scale =
+ * f16((max - minimum) / 15) (the fp32 product with 1/15), code = round((x -
+ * minimum) * (1 / scale)) in 0..15, what a code stands for is minimum + scale *
+ * code.  A group that holds a NaN is NaN. */
+size_t grinqh_kv4_record_bytes(int head_dim, int group);
+
+/* Writes the keys and values of `tokens` tokens at their slots (int64 [tokens],
+ * device; slot = page * page_size + place).  A slot outside the cache (-1:
+ * padding) is skipped.  No two tokens may have the same slot. */
+int grinqh_kv4_store(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                     const int64_t* slots, int64_t tokens, void* cache, int64_t pages, int kv_heads, int page_size,
+                     int head_dim, int group, int dtype, void* stream);
+
+/* Reads slots back: k_out and v_out [tokens][kv_heads][head_dim]; a slot outside
+ * the cache gives zeros. */
+int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                    const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int dtype, void* stream);
+
+/* out[s] = softmax(scale q[s] k^T) v over the first lengths[s] tokens of sequence
+ * s, whose pages are page_table[s][0 .. table_width - 1] (int32, rows table_stride
+ * apart; entries past a sequence's last page are not read).  heads is a
+ * multiple of kv_heads.  A length of 0 gives zeros; a length past the table or a
+ * page outside the cache makes the sequence's results NaN.  max_length plans how
+ * a sequence is split over blocks; longer lengths are right, only slower.
+ * scale > 0.  The workspace (grinqh_kv4_attention_workspace_bytes, 256-byte
+ * aligned, needs no initial contents) is for one call at a time. */
+size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t max_length);
+int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
+                         int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                         const int32_t* page_table, int64_t table_stride, int table_width, const int32_t* lengths,
+                         int64_t max_length, float scale, void* out, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Causal attention over packed sequences: rows q_ends[s] .. q_ends[s + 1] - 1
+ * of q attend to keys k_ends[s] .. k_ends[s + 1] - 1 (int32 [seqs + 1] each,
+ * device, ascending; the same array for plain prompts).  The last rows are
+ * aligned with the last keys: row i of R sees keys 0 .. i + (K - R) of K, none
+ * when that is negative (zeros).  Rows behind the last sequence give zeros.
+ * Offsets are limited to the tensors.  scale > 0. */
+int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                            int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* q_ends,
+                            const int32_t* k_ends, int64_t seqs, int64_t q_tokens, int64_t k_tokens, int heads,
+                            int kv_heads, int head_dim, float scale, void* out, int dtype, void* stream);
+
 /* Benchmark instrumentation; no counterpart in the reference.  Arms a one-shot
  * timer: in the next grinqh_gemm_or_gemv / grinqh_gemv_batch_union /
  * grinqh_prefill_dense call (from any thread), the dispatch of its first main

@@ -3,12 +3,14 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <cfloat>
 #include <cstdlib>
 #include <cstring>
 
 #include <mutex>
 
 #include "grinqh_common.h"
+#include "attention_launch.h"
 #include "grinqh_launch.h"
 
 using namespace grinqh;
@@ -500,6 +502,33 @@ int scratch_on_current_device(void** out, hipStream_t st) {
   return GRINQH_OK;
 }
 
+// ---- argument checks of the attention entry points
+
+bool valid_head(int head_dim, int group) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+         (group == 32 || group == 64 || group == 128 || group == 256) && group <= head_dim;
+}
+bool valid_heads(int heads, int kv_heads) { return kv_heads > 0 && heads > 0 && heads % kv_heads == 0; }
+bool valid_scale(float scale) { return scale > 0.f && scale <= FLT_MAX; }
+
+bool valid_cache(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group) {
+  const int sub = page_size / 16;
+  if (!valid_head(head_dim, group) || kv_heads <= 0 || page_size < 16 || page_size % 16 != 0 || (sub & (sub - 1)) != 0)
+    return false;
+  return pages == 0 || (pages > 0 && cache != nullptr && aligned(cache, 64));
+}
+Kv4Cache kv4_cache(void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group) {
+  return Kv4Cache{static_cast<uint8_t*>(cache), pages, kv_heads, page_size / 16, head_dim, head_dim / group};
+}
+
+// Rows of 16-byte loads; a prompt tile's byte offsets (64 tokens) fit 31 bits.
+bool head_rows(const void* p, int64_t token, int64_t head, HeadRows* out) {
+  constexpr int64_t kMostDistance = (int64_t)1 << 23;
+  *out = HeadRows{static_cast<const uint16_t*>(p), token, head};
+  return p != nullptr && aligned(p, 16) && token % 8 == 0 && head % 8 == 0 && token >= 0 && head >= 0 &&
+         token <= kMostDistance && head <= kMostDistance;
+}
+
 }  // namespace
 
 extern "C" {
@@ -704,6 +733,102 @@ int grinqh_expire_tile_waits(int on) {
   const int before = t_expire_waits;
   t_expire_waits = on != 0 ? 1 : 0;
   return before;
+}
+
+// ---- attention
+
+size_t grinqh_kv4_record_bytes(int head_dim, int group) {
+  return valid_head(head_dim, group) ? (size_t)kv4_record_bytes(head_dim, head_dim / group) : 0;
+}
+
+int grinqh_kv4_store(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                     const int64_t* slots, int64_t tokens, void* cache, int64_t pages, int kv_heads, int page_size,
+                     int head_dim, int group, int dtype, void* stream) {
+  if (!valid_dtype(dtype) || tokens < 0 || !valid_cache(cache, pages, kv_heads, page_size, head_dim, group))
+    return GRINQH_ERR_INVALID;
+  if (tokens == 0 || pages == 0) return GRINQH_OK;
+  HeadRows kr, vr;
+  if (!head_rows(k, k_token, k_head, &kr) || !head_rows(v, v_token, v_head, &vr) || slots == nullptr)
+    return GRINQH_ERR_INVALID;
+  return launch_kv4_store(kr, vr, slots, tokens, kv4_cache(cache, pages, kv_heads, page_size, head_dim, group), dtype,
+                          as_stream(stream));
+}
+
+int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                    const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int dtype, void* stream) {
+  if (!valid_dtype(dtype) || tokens < 0 || !valid_cache(cache, pages, kv_heads, page_size, head_dim, group))
+    return GRINQH_ERR_INVALID;
+  if (tokens == 0) return GRINQH_OK;
+  if (slots == nullptr || k_out == nullptr || v_out == nullptr || !aligned(k_out, 16) || !aligned(v_out, 16))
+    return GRINQH_ERR_INVALID;
+  return launch_kv4_load(kv4_cache(const_cast<void*>(cache), pages, kv_heads, page_size, head_dim, group), slots,
+                         tokens, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), dtype,
+                         as_stream(stream));
+}
+
+size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t max_length) {
+  if (seqs <= 0 || seqs > INT32_MAX || max_length > INT32_MAX || !valid_heads(heads, kv_heads)) return 0;
+  return plan_kv4(seqs, heads, kv_heads, head_dim, max_length).workspace;
+}
+
+int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
+                         int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                         const int32_t* page_table, int64_t table_stride, int table_width, const int32_t* lengths,
+                         int64_t max_length, float scale, void* out, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_scale(scale) || seqs < 0 || seqs > INT32_MAX ||
+      !valid_cache(cache, pages, kv_heads, page_size, head_dim, group) || table_width < 0 || max_length < 0 ||
+      max_length > INT32_MAX)
+    return GRINQH_ERR_INVALID;
+  if (seqs == 0) return GRINQH_OK;
+  // every page index is checked against `pages`; with none there is nothing a bad one could stand for
+  if (pages == 0) table_width = 0;
+  Kv4Params p;
+  if (!head_rows(q, q_token, q_head, &p.q) || lengths == nullptr || out == nullptr || !aligned(out, 16) ||
+      (table_width > 0 && page_table == nullptr) || (int64_t)table_width * page_size > INT32_MAX)
+    return GRINQH_ERR_INVALID;
+  p.out = static_cast<uint16_t*>(out);
+  p.cache = kv4_cache(const_cast<void*>(cache), pages, kv_heads, page_size, head_dim, group);
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.lengths = lengths;
+  p.seqs = (int)seqs;
+  p.heads = heads;
+  p.scale = scale;
+  p.plan = plan_kv4(seqs, heads, kv_heads, head_dim, max_length);
+  p.partial = static_cast<float*>(workspace);
+  if (p.plan.workspace > 0 && (workspace == nullptr || workspace_bytes < p.plan.workspace || !aligned(workspace, 256)))
+    return GRINQH_ERR_WORKSPACE;
+  return launch_kv4_attention(p, dtype, as_stream(stream));
+}
+
+int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                            int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* q_ends,
+                            const int32_t* k_ends, int64_t seqs, int64_t q_tokens, int64_t k_tokens, int heads,
+                            int kv_heads, int head_dim, float scale, void* out, int dtype, void* stream) {
+  if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_head(head_dim, head_dim) || !valid_scale(scale) ||
+      seqs < 0 || seqs >= INT32_MAX || q_tokens < 0 || q_tokens > INT32_MAX || k_tokens < 0 || k_tokens > INT32_MAX)
+    return GRINQH_ERR_INVALID;
+  if (q_tokens == 0) return GRINQH_OK;
+  PromptParams p;
+  if (!head_rows(q, q_token, q_head, &p.q) || out == nullptr || !aligned(out, 16) || q_ends == nullptr ||
+      k_ends == nullptr)
+    return GRINQH_ERR_INVALID;
+  p.k = p.v = HeadRows{nullptr, 0, 0};
+  if (k_tokens > 0 && (!head_rows(k, k_token, k_head, &p.k) || !head_rows(v, v_token, v_head, &p.v)))
+    return GRINQH_ERR_INVALID;
+  p.out = static_cast<uint16_t*>(out);
+  p.ends = q_ends;
+  p.key_ends = k_ends;
+  p.q_tokens = q_tokens;
+  p.k_tokens = k_tokens;
+  p.seqs = (int)seqs;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.head_size = head_dim;
+  p.scale = scale;
+  return launch_prompt_attention(p, dtype, as_stream(stream));
 }
 
 }  // extern "C"
