@@ -226,17 +226,18 @@ int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_siz
 /* out[s] = softmax(scale q[s] k^T) v over the first lengths[s] tokens of sequence
  * s, whose pages are page_table[s][0 .. table_width - 1] (int32, rows table_stride
  * apart; entries past a sequence's last page are not read).  heads is a
- * multiple of kv_heads.  A length of 0 gives zeros; a length past the table or a
- * page outside the cache makes the sequence's results NaN.  max_length plans how
- * a sequence is split over blocks; longer lengths are right, only slower.
- * scale > 0.  The workspace (grinqh_kv4_attention_workspace_bytes, 256-byte
- * aligned, needs no initial contents) is for one call at a time. */
-size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t max_length);
+ * multiple of kv_heads; scale > 0.  A length of 0 gives zeros; a length past the
+ * table or a page outside the cache makes the sequence's results NaN.  The
+ * lengths are read on the device, where the blocks share the work out.  The
+ * workspace (grinqh_kv4_attention_workspace_bytes for a capacity of table_width *
+ * page_size tokens, 256-byte aligned) is zero-filled once before its first use
+ * (every call leaves its counters zero again); calls that share one must be
+ * ordered (same stream). */
+size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t capacity);
 int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
                          int64_t pages, int kv_heads, int page_size, int head_dim, int group,
                          const int32_t* page_table, int64_t table_stride, int table_width, const int32_t* lengths,
-                         int64_t max_length, float scale, void* out, int dtype, void* workspace,
-                         size_t workspace_bytes, void* stream);
+                         float scale, void* out, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Causal attention over packed sequences: rows q_ends[s] .. q_ends[s + 1] - 1
  * of q attend to keys k_ends[s] .. k_ends[s + 1] - 1 (int32 [seqs + 1] each,

@@ -256,18 +256,41 @@ def test_decode_many_query_heads(per, d):
     _check_decode(ga.kv4_attention(q, cache, table, lengths), q, seqs, 64, "f16")
 
 
-@pytest.mark.parametrize("max_length", [None, 0, 1, 100, 3000, 10 ** 9])
-@pytest.mark.parametrize("seqs", [1, 3])
-def test_decode_split_lengths(max_length, seqs):
-    """few sequences are split over blocks; a bound that is too small or far too large changes nothing"""
+@pytest.mark.parametrize("lens", [[2777], [2777, 40, 0], [9000, 1, 513], [0, 0, 5000, 0], [512, 513, 544, 545]])
+@pytest.mark.parametrize("hkv,per", [(2, 4), (1, 16), (1, 33), (3, 1)])
+def test_decode_split_lengths(lens, hkv, per):
+    """few sequences are shared by several blocks; a table with room for more changes nothing but the plan"""
     from grinqh import attention as ga
     rng = np.random.default_rng(17)
-    lens = [2777, 40, 0][:seqs]
-    cache, table, lengths, kv = _paged(rng, lens, 2, 128, 16, 128, "bf16")
-    q = _randn(rng, seqs, 8, 128, dtype="bf16")
-    wide = torch.nn.functional.pad(table, (0, 700), value=-1)  # a table with room for more
+    cache, table, lengths, kv = _paged(rng, lens, hkv, 128, 16, 128, "bf16")
+    q = _randn(rng, len(lens), hkv * per, 128, dtype="bf16")
+    wide = torch.nn.functional.pad(table, (0, 700), value=-1)
     for tab in (table, wide):
-        _check_decode(ga.kv4_attention(q, cache, tab, lengths, max_length=max_length), q, kv, 128, "bf16")
+        for _ in range(2):  # the counters are zero again after a call
+            _check_decode(ga.kv4_attention(q, cache, tab, lengths), q, kv, 128, "bf16")
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65, 130, 700])
+def test_decode_many_sequences(seqs):
+    from grinqh import attention as ga
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(0, 60, seqs)
+    lens[seqs // 3], lens[seqs // 2], lens[-1] = 3000, 0, 700
+    cache, table, lengths, kv = _paged(rng, lens.tolist(), 1, 64, 16, 64, "f16")
+    q = _randn(rng, seqs, 2, 64)
+    _check_decode(ga.kv4_attention(q, cache, table, lengths), q, kv, 64, "f16")
+
+
+def test_decode_more_units_than_counters():
+    """beyond 2^15 (sequence, head) pairs no sequence is shared between blocks"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(2)
+    cache, table, lengths, kv = _paged(rng, [900, 33], 8, 64, 16, 64, "f16")
+    pick = torch.arange(5000).cuda() % 2
+    q = _randn(rng, 2, 8, 64)
+    out = ga.kv4_attention(q[pick], cache, table[pick], lengths[pick])
+    assert torch.equal(out, out[:2][pick])
+    _check_decode(out[:2], q, kv, 64, "f16")
 
 
 @pytest.mark.parametrize("tokens", [48, 4000])
@@ -612,7 +635,6 @@ def test_refusals():
         lambda: ga.kv4_attention(q, cache, table, lengths, scale=0.0),
         lambda: ga.kv4_attention(q, cache, table, lengths, scale=float("nan")),
         lambda: ga.kv4_attention(q, cache, table, lengths, scale=-1.0),
-        lambda: ga.kv4_attention(q, cache, table, lengths, max_length=-1),
         lambda: ga.prompt_attention(q, z(3, 3, 128), z(3, 3, 128), lengths),
         lambda: ga.prompt_attention(z(3, 8, 96), z(3, 8, 96), z(3, 8, 96), lengths),
         lambda: ga.prompt_attention(q, k, z(3, 2, 64), lengths),

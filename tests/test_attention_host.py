@@ -68,20 +68,20 @@ def test_c_entry_points_refuse(lib):
         assert store(**kw) == 1, kw
     assert store(tokens=0) == 0 and store(pages=0, cache=None) == 0
 
-    def attend(q=p, seqs=2, heads=8, kv=2, table=p, width=4, lengths=p, most=64, scale=0.1, out=p, dt=0, ws=None, n=0):
+    def attend(q=p, seqs=2, heads=8, kv=2, table=p, width=4, lengths=p, scale=0.1, out=p, dt=0, ws=None, n=0):
         return lib.grinqh_kv4_attention(q, 1024, 128, seqs, heads, p, 8, kv, 16, 128, 128, table, width, width, lengths,
-                                        most, scale, out, dt, ws, n, None)
+                                        scale, out, dt, ws, n, None)
 
     for kw in ({"q": None}, {"q": bad_p}, {"seqs": -1}, {"heads": 7}, {"heads": 0}, {"kv": 0}, {"table": None},
-               {"width": -1}, {"width": 1 << 30}, {"lengths": None}, {"most": -1}, {"most": 1 << 31}, {"scale": 0.0},
+               {"width": -1}, {"width": 1 << 30}, {"lengths": None}, {"scale": 0.0},
                {"scale": float("nan")}, {"scale": float("inf")}, {"out": None}, {"out": bad_p}, {"dt": 5}):
         assert attend(**kw) == 1, kw
     assert attend(seqs=0) == 0
-    assert attend(most=100000, width=100000) == 3  # no workspace
-    need = lib.grinqh_kv4_attention_workspace_bytes(2, 8, 2, 128, 100000)
+    assert attend(width=10000) == 3  # no workspace
+    need = lib.grinqh_kv4_attention_workspace_bytes(2, 8, 2, 128, 160000)
     assert need > 0
-    assert attend(most=100000, width=100000, ws=p, n=need - 1) == 3
-    assert attend(most=100000, width=100000, ws=bad_p, n=need) == 3
+    assert attend(width=10000, ws=p, n=need - 1) == 3
+    assert attend(width=10000, ws=bad_p, n=need) == 3
 
     def prompt(q=p, k=p, heads=8, kv=2, d=128, rows=5, keys=5, ends=p, seqs=1, scale=0.1, out=p, dt=0):
         return lib.grinqh_prompt_attention(q, 1024, 128, k, 256, 128, p, 256, 128, ends, p, seqs, rows, keys, heads, kv,
@@ -95,7 +95,10 @@ def test_c_entry_points_refuse(lib):
 
 def test_workspace_query(lib):
     q = lib.grinqh_kv4_attention_workspace_bytes
-    assert q(1000, 32, 8, 128, 100000) == 0     # enough sequences to fill the GPU
-    assert q(1, 32, 8, 128, 1) == 0
-    assert q(0, 32, 8, 128, 100) == 0 and q(1, 5, 2, 128, 100) == 0
-    assert q(1, 32, 8, 128, 131072) % (32 * 130 * 4) == 0
+    counters = 4 << 15
+    assert q(1, 32, 8, 128, 1024) == 0          # one run of 32 steps
+    assert q(1, 32, 8, 128, 1025) == counters + (8 + 8) * (4 * 128 + 32) * 4
+    assert q(1, 32, 8, 128, 131072) == counters + (8 + 256) * (4 * 128 + 32) * 4
+    assert q(1, 64, 1, 64, 131072) == counters + (4 + 256) * (16 * 64 + 32) * 4   # 4 tiles of 16 query heads
+    assert q(5000, 32, 8, 128, 131072) == 0     # more units than counters: none is shared
+    assert q(0, 32, 8, 128, 100) == 0 and q(1, 5, 2, 128, 100) == 0 and q(1, 4, 2, 128, 0) == 0

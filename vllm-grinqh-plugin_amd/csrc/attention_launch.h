@@ -21,7 +21,7 @@ struct HeadRows {
 struct Kv4Cache {
   uint8_t* p;
   int64_t pages;
-  int heads, sub, head_size, groups;
+  int heads, sub, head_size, groups;  // sub: a power of two
 };
 
 constexpr int kv4_record_bytes(int head_size, int groups) { return 16 * head_size + 64 * (groups + 1); }
@@ -31,13 +31,18 @@ int launch_kv4_store(HeadRows k, HeadRows v, const int64_t* slots, int64_t token
 int launch_kv4_load(const Kv4Cache& cache, const int64_t* slots, int64_t tokens, uint16_t* k, uint16_t* v, int dtype,
                     hipStream_t st);
 
-// How kv4_attention splits its sequences: runs of `chunk` steps of 32 tokens,
-// at most `splits` of them.
+// How kv4_attention shares its work out (find_share in kv4.hip); the lengths are
+// known on the device only.
+constexpr int64_t kKv4Counters = 1 << 15;  // units that can be shared by several blocks, one counter each
 struct Kv4Plan {
-  int splits, chunk;
-  size_t workspace;  // bytes, 0 if splits == 1
+  int waves;         // per block: 4 or 8
+  int blocks;        // blocks that the steps of all units are shared out over
+  int least, most;   // steps of a run at least, runs of a unit at most
+  int slot;          // floats of a run's result in the workspace
+  int64_t grid;      // blocks launched: one per unit and those that share one
+  size_t workspace;  // bytes, 0 if no unit is shared
 };
-Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t max_length);
+Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity);
 
 struct Kv4Params {
   HeadRows q;
@@ -48,9 +53,12 @@ struct Kv4Params {
   int table_width;
   const int32_t* lengths;
   int seqs, heads;
+  int sub_shift;  // log2(cache.sub)
   float scale;
   Kv4Plan plan;
-  float* partial;  // [seqs][heads][splits][head size + 2]
+  int units;          // per sequence: key/value heads x tiles of their query heads
+  uint32_t* counters;  // [kKv4Counters], zero on entry and on exit
+  float* partial;      // [plan.grid][plan.slot]
 };
 int launch_kv4_attention(const Kv4Params& p, int dtype, hipStream_t st);
 

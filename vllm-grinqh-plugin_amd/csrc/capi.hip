@@ -766,19 +766,17 @@ int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_siz
                          as_stream(stream));
 }
 
-size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t max_length) {
-  if (seqs <= 0 || seqs > INT32_MAX || max_length > INT32_MAX || !valid_heads(heads, kv_heads)) return 0;
-  return plan_kv4(seqs, heads, kv_heads, head_dim, max_length).workspace;
+size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t capacity) {
+  if (seqs <= 0 || seqs > INT32_MAX || capacity <= 0 || capacity > INT32_MAX || !valid_heads(heads, kv_heads)) return 0;
+  return plan_kv4(seqs, heads, kv_heads, head_dim, capacity).workspace;
 }
 
 int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
                          int64_t pages, int kv_heads, int page_size, int head_dim, int group,
                          const int32_t* page_table, int64_t table_stride, int table_width, const int32_t* lengths,
-                         int64_t max_length, float scale, void* out, int dtype, void* workspace,
-                         size_t workspace_bytes, void* stream) {
+                         float scale, void* out, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_scale(scale) || seqs < 0 || seqs > INT32_MAX ||
-      !valid_cache(cache, pages, kv_heads, page_size, head_dim, group) || table_width < 0 || max_length < 0 ||
-      max_length > INT32_MAX)
+      !valid_cache(cache, pages, kv_heads, page_size, head_dim, group) || table_width < 0)
     return GRINQH_ERR_INVALID;
   if (seqs == 0) return GRINQH_OK;
   // every page index is checked against `pages`; with none there is nothing a bad one could stand for
@@ -789,6 +787,7 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
     return GRINQH_ERR_INVALID;
   p.out = static_cast<uint16_t*>(out);
   p.cache = kv4_cache(const_cast<void*>(cache), pages, kv_heads, page_size, head_dim, group);
+  p.sub_shift = __builtin_ctz((unsigned)p.cache.sub);
   p.table = page_table;
   p.table_stride = table_stride;
   p.table_width = table_width;
@@ -796,8 +795,10 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
   p.seqs = (int)seqs;
   p.heads = heads;
   p.scale = scale;
-  p.plan = plan_kv4(seqs, heads, kv_heads, head_dim, max_length);
-  p.partial = static_cast<float*>(workspace);
+  p.units = kv_heads * ((heads / kv_heads + 15) / 16);
+  p.plan = plan_kv4(seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size);
+  p.counters = static_cast<uint32_t*>(workspace);
+  p.partial = reinterpret_cast<float*>(p.counters + kKv4Counters);
   if (p.plan.workspace > 0 && (workspace == nullptr || workspace_bytes < p.plan.workspace || !aligned(workspace, 256)))
     return GRINQH_ERR_WORKSPACE;
   return launch_kv4_attention(p, dtype, as_stream(stream));

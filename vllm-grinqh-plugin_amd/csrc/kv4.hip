@@ -25,6 +25,7 @@
 
 #include "attention_launch.h"
 #include "grinqh_common.h"
+#include "splitk_complete.h"
 
 namespace grinqh {
 
@@ -32,8 +33,11 @@ namespace {
 
 constexpr float kLimit = 65504.f;  // largest finite fp16
 
+// one v_cvt_pk_f16_f32 (round to nearest even)
 __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
-  return (uint32_t)f32_to_f16_bits(lo) | ((uint32_t)f32_to_f16_bits(hi) << 16);
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), f16x2_t));
 }
 __device__ __forceinline__ float half_lo(uint32_t w) { return f16_bits_to_f32((uint16_t)w); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return f16_bits_to_f32((uint16_t)(w >> 16)); }
@@ -153,52 +157,152 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Cache cache, const int
 
 // ---------------------------------------------------------------- attention, one token per sequence
 
-constexpr int kWaves = 4;       // per block
 constexpr int kRows = 16;       // query heads of one key/value head per block
+constexpr int kRuns = 256;      // most blocks that share one sequence and head
 constexpr float kLow = -1e30f;  // running reference before the first token (finite: -inf - -inf would be NaN)
 
-// What one wave holds of 32 tokens (two records).
+// Inclusive sum over the lanes of a wave (row shifts, then the rows' totals).
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int x = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                              decltype(rows)::value, 0xf, false);
+    v += __builtin_bit_cast(T, x);
+  };
+  using I = std::integral_constant<int, 0xf>;
+  step(std::integral_constant<int, 0x111>{}, I{});
+  step(std::integral_constant<int, 0x112>{}, I{});
+  step(std::integral_constant<int, 0x114>{}, I{});
+  step(std::integral_constant<int, 0x118>{}, I{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return v;
+}
+
+// Which run of 32-token steps a block takes.
+struct Share {
+  int seq, unit;         // unit: key/value head and tile of its query heads
+  int first, last;       // steps
+  int run, runs;         // this is run `run` of the unit's
+  int length;            // of the sequence, in tokens
+  bool bad;              // it is longer than the page table
+};
+
+__device__ __forceinline__ int length_of(const Kv4Params& p, int seq, bool& bad) {
+  const int64_t capacity = (int64_t)p.table_width << (p.sub_shift + 4);
+  const int length = max(p.lengths[seq], 0);
+  bad = length > capacity;
+  return bad ? (int)capacity : length;
+}
+// Every block plans by itself from the lengths, which only the device knows:
+// the steps of all sequences and heads shared out over plan.blocks, in runs of
+// at least plan.least steps that never leave their sequence, all runs of a
+// sequence alike.  A lane sums up seqs / 64 sequences, a scan over the lanes
+// finds the block's.  False: more blocks than runs.
+__device__ __forceinline__ bool find_share(const Kv4Params& p, int id, int lane, Share& s) {
+  if (p.plan.most == 1) {
+    s.seq = id / p.units;
+    s.unit = id - s.seq * p.units;
+    s.length = length_of(p, s.seq, s.bad);
+    s.run = s.first = 0;
+    s.runs = 1;
+    s.last = (s.length + 31) >> 5;
+    return true;
+  }
+  const int group = (p.seqs + 63) >> 6, s0 = lane * group;
+  bool bad = false;
+  const int mine = lane < p.seqs ? length_of(p, lane, bad) : 0;  // all there is with up to 64 sequences
+  const uint64_t bads = __ballot(bad);
+  auto steps_of = [&](int i) {  // of the lane's i-th sequence
+    bool b;
+    return ((group == 1 ? mine : length_of(p, s0 + i, b)) + 31) >> 5;
+  };
+  float steps = 0.f;
+  for (int i = 0; i < group; ++i)
+    if (s0 + i < p.seqs) steps += (float)steps_of(i);
+  const float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(steps)), 63));
+  const int chunk = max(p.plan.least, (int)ceilf(fminf(total * (float)p.units / (float)p.plan.blocks, 0x1p26f)));
+  auto runs_of = [&](int n) { return min(max((n + chunk - 1) / chunk, 1), p.plan.most); };
+  int runs = 0;
+  for (int i = 0; i < group; ++i)
+    if (s0 + i < p.seqs) runs += runs_of(steps_of(i)) * p.units;
+  const int upto = wave_scan(runs);
+  const uint64_t after = __ballot(upto > id);
+  if (after == 0) return false;
+  const int owner = __builtin_ctzll(after);
+  int rest = id - __builtin_amdgcn_readlane(upto - runs, owner);
+  int seq = owner * group, k = 1;
+  for (;; ++seq) {
+    if (group == 1) {
+      s.length = __builtin_amdgcn_readlane(mine, seq);
+      s.bad = (bads >> seq) & 1;
+    } else {
+      s.length = __builtin_amdgcn_readfirstlane(length_of(p, seq, s.bad));
+    }
+    k = runs_of((s.length + 31) >> 5);
+    if (rest < k * p.units) break;
+    rest -= k * p.units;
+  }
+  const int n = (s.length + 31) >> 5, per = (n + k - 1) / k;
+  s.seq = seq;
+  s.runs = k;
+  s.unit = rest / k;
+  s.run = rest - s.unit * k;
+  s.first = s.run * per;
+  s.last = min(s.first + per, n);
+  return true;
+}
+
+// What a lane holds of 32 tokens (two records).  The parameters are loaded once
+// per wave, a word or a few per lane, and handed round through LDS when they
+// are used: a lane needs those of 8 tokens, 8 (G + 1) words, and the prefetch
+// would have no registers for them.
 template <int D, int G>
 struct Tokens {
+  static constexpr int kParams = 32 * (G + 1);  // words
   uint32_t k[2][D / 32];
-  u32x4_t kp[2][G];
   u32x4_t v[2][D < 128 ? 1 : D / 128];
-  u32x4_t vp[2];
+  uint32_t par[(kParams + 63) / 64];
 };
 
 template <int D, int G>
-__device__ __forceinline__ void load_tokens(Tokens<D, G>& t, int r, const uint8_t* __restrict__ rec, int lane) {
+__device__ __forceinline__ void load_tokens(Tokens<D, G>& t, const uint8_t* __restrict__ rec0,
+                                            const uint8_t* __restrict__ rec1, int lane) {
   const int n = lane & 15, quad = lane >> 4;
-  constexpr int W = D / 32;
-  const uint8_t* kb = rec + n * (D / 2) + quad * (D / 8);
-  if constexpr (W == 2) {
-    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(kb);
-    t.k[r][0] = x[0];
-    t.k[r][1] = x[1];
-  } else {
+  constexpr int W = D / 32, PER = 16 * (G + 1);
 #pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(kb + 4 * i);
+  for (int r = 0; r < 2; ++r) {
+    const uint8_t* rec = r == 0 ? rec0 : rec1;
+    const uint8_t* kb = rec + (uint32_t)(n * (D / 2) + quad * (D / 8));
+    if constexpr (W == 2) {
+      const u32x2_t x = *reinterpret_cast<const u32x2_t*>(kb);
+      t.k[r][0] = x[0];
+      t.k[r][1] = x[1];
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t.k[r][i + j] = x[j];
+      for (int i = 0; i < W; i += 4) {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(kb + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t.k[r][i + j] = x[j];
+      }
     }
+    const uint8_t* vb = rec + (uint32_t)(8 * D + 64 * G + (D < 128 ? n & 7 : n) * 64 + 16 * quad);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(t.v[r]) / 16); ++i) t.v[r][i] = *reinterpret_cast<const u32x4_t*>(vb + 1024 * i);
   }
 #pragma unroll
-  for (int g = 0; g < G; ++g) t.kp[r][g] = *reinterpret_cast<const u32x4_t*>(rec + 8 * D + 64 * g + 16 * quad);
-  const uint8_t* vb = rec + 8 * D + 64 * G;
-  if constexpr (D < 128) {
-    t.v[r][0] = *reinterpret_cast<const u32x4_t*>(vb + (n & 7) * 64 + 16 * quad);
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 128; ++i)
-      t.v[r][i] = *reinterpret_cast<const u32x4_t*>(vb + (n + 16 * i) * 64 + 16 * quad);
+  for (int j = 0; j < (int)(sizeof(t.par) / 4); ++j) {
+    const int i = min(lane + 64 * j, 2 * PER - 1), w = i < PER ? i : i - PER;
+    const uint32_t at = w < 16 * G ? 8 * D + 4 * w : 16 * D + 4 * w;
+    t.par[j] = *reinterpret_cast<const uint32_t*>((i < PER ? rec0 : rec1) + at);
   }
-  t.vp[r] = *reinterpret_cast<const u32x4_t*>(rec + 16 * D + 64 * G + 16 * quad);
 }
 
 // Block = one sequence, one key/value head (up to 16 of its query heads) and
 // one run of tokens; its waves take 32-token steps in turn, each with a softmax
-// of its own, joined at the end (and with other blocks' by kv4_join_kernel).
+// of its own, joined at the end.  Where a sequence is shared by several blocks,
+// each leaves its result in the workspace and the one that arrives last joins
+// them, in their order.
 //
 // S^T = K Q^T leaves a lane with one query row and 8 of the 32 tokens, which
 // is the B operand of O^T = V^T P^T: nothing crosses lanes in the loop.  With
@@ -211,41 +315,81 @@ __device__ __forceinline__ void load_tokens(Tokens<D, G>& t, int r, const uint8_
 // the values' size.  Queries are brought to 2^13 <= max < 2^14 by a power of two
 // (exact), so fp16 holds them for both types and the nibbles that come out
 // 16-fold can be undone on the query's side.
-template <typename DT, int D, int G>
-__global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Params p) {
-  constexpr int R = kv4_record_bytes(D, G), W = D / 32, M_TILES = D < 128 ? 1 : D / 128, SLOTS = D < 128 ? 4 : 8;
-  __shared__ float s_o[kWaves][kRows][D + 4];
+template <typename DT, int D, int G, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_kernel(const Kv4Params p) {
+  constexpr int kWaves = WAVES, kThreads = 64 * WAVES;
+  constexpr int R = kv4_record_bytes(D, G), W = D / 32, M_TILES = D < 128 ? 1 : D / 128, ACCS = D < 128 ? 4 : 8;
+  __shared__ union {
+    float o[kWaves][kRows][D + 4];
+    struct {
+      float weight[kRows][kRuns];
+      f32x4_t sum[kThreads];
+    } join;
+  } sh;
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows], s_off[kWaves][kRows];
+  __shared__ __align__(16) uint32_t s_par[kWaves][Tokens<D, G>::kParams];
+  __shared__ int s_last;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = p.heads / p.cache.heads, tiles = (per + kRows - 1) / kRows;
-  int id = blockIdx.x;
-  const int split = id % p.plan.splits;
-  id /= p.plan.splits;
-  const int tile = id % tiles;
-  id /= tiles;
-  const int kvh = id % p.cache.heads, seq = id / p.cache.heads;
+  Share share;
+  if (!find_share(p, blockIdx.x, lane, share)) return;
+  const int seq = share.seq, first = share.first, last = share.last;
+  const int per = p.heads / p.cache.heads, tiles = p.units / p.cache.heads;
+  const int kvh = share.unit / tiles, tile = share.unit - kvh * tiles;
   const int h0 = kvh * per + tile * kRows, rows = min(kRows, per - tile * kRows);
+  const int length = share.length;
+  bool bad = share.bad;
 
-  const int64_t capacity = (int64_t)p.table_width * p.cache.sub * 16;
-  int length = max(p.lengths[seq], 0);
-  bool bad = (int64_t)length > capacity;
-  if (bad) length = (int)capacity;
-  const int steps = (length + 31) >> 5;
-  const int first = split * p.plan.chunk;
-  const int last = split + 1 == p.plan.splits ? steps : min(steps, first + p.plan.chunk);
-  if (split > 0 && first >= steps) return;
-
-  // queries: row n, channels 32 s + 8 quad + e
   u32x4_t qf[W];
+  {
+    const uint16_t* q = p.q.p + (int64_t)seq * p.q.token + (int64_t)(h0 + min(n, rows - 1)) * p.q.head + 8 * quad;
+#pragma unroll
+    for (int s = 0; s < W; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 32 * s);
+  }
+  // Two slots of tokens: one is computed while the other's loads are in flight
+  // (8 waves per CU then have 35 KB on their way; a third slot gave nothing).
+  constexpr int SLOTS = 2;
+  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
+  const int last_rec = max((length - 1) >> 4, 0);
+  auto record = [&](int step, int r, int page) -> const uint8_t* {
+    if ((uint32_t)page >= (uint64_t)p.cache.pages) {
+      bad = true;
+      page = 0;
+    }
+    const int rec = min(2 * step + r, last_rec);
+    return p.cache.p + ((((int64_t)page * p.cache.heads + kvh) << p.sub_shift) + (rec & (p.cache.sub - 1))) * R;
+  };
+  Tokens<D, G> slots[SLOTS];
+  const int begin = first + wave;
+  // Pages: a lane holds one of the next 64 records', loaded once for ROUND steps
+  // (a load per step would sit behind the tokens' loads, and waiting for it would
+  // be waiting for them).  Past the end a step stands for the last one: a load
+  // under a condition would make every wait a wait for all loads.
+  constexpr int ROUND = 27 / SLOTS * SLOTS;  // ROUND + SLOTS <= 32
+  auto pages_from = [&](int step) {
+    const int at = min(step + (lane >> 1) * kWaves, last - 1);
+    return table[min(2 * at + (lane & 1), last_rec) >> p.sub_shift];
+  };
+  int pages = 0;
+  auto fetch = [&](Tokens<D, G>& t, int step, int place) {
+    const int at = min(step, last - 1);
+    load_tokens<D, G>(t, record(at, 0, __builtin_amdgcn_readlane(pages, 2 * place)),
+                      record(at, 1, __builtin_amdgcn_readlane(pages, 2 * place + 1)), lane);
+  };
+  if (begin < last) {
+    pages = pages_from(begin);
+    asm volatile("" : "+v"(pages));
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) fetch(slots[i], begin + i * kWaves, i);
+  }
+
   float qsum[G], qs;
   {
-    const uint16_t* q = p.q.p + (int64_t)seq * p.q.token + (int64_t)(h0 + min(n, rows - 1)) * p.q.head;
     float x[W][8];
     float mx = 0.f;
 #pragma unroll
     for (int s = 0; s < W; ++s) {
-      const u32x4_t in = *reinterpret_cast<const u32x4_t*>(q + 32 * s + 8 * quad);
+      const u32x4_t in = qf[s];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[s][e] = n < rows ? to_f32<DT>((uint16_t)(in[e >> 1] >> (16 * (e & 1)))) : 0.f;
@@ -280,41 +424,28 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
     qs = ldexpf(p.scale * 1.44269504088896f, 24 - ex);  // logits in powers of two
   }
 
-  f32x4_t O[M_TILES][SLOTS];
+  f32x4_t O[M_TILES][ACCS];
 #pragma unroll
   for (int i = 0; i < M_TILES; ++i)
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) O[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < ACCS; ++j) O[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float M = kLow, L = 0.f, off = 0.f;
 
-  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
-  const int last_rec = max((length - 1) >> 4, 0);
-  auto record = [&](int step, int r) -> const uint8_t* {
-    const int rec = min(2 * step + r, last_rec);
-    int page = table[rec / p.cache.sub];
-    if ((uint32_t)page >= (uint64_t)p.cache.pages) {
-      bad = true;
-      page = 0;
-    }
-    return p.cache.p + (((int64_t)page * p.cache.heads + kvh) * p.cache.sub + (rec & (p.cache.sub - 1))) * R;
-  };
-
-  for (int step = first + wave; step < last; step += kWaves) {
-    Tokens<D, G> t;
-    load_tokens<D, G>(t, 0, record(step, 0), lane);
-    load_tokens<D, G>(t, 1, record(step, 1), lane);
-
-    float z[8], vs[8], vm[8];
+  auto compute = [&](const Tokens<D, G>& t, int step) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(t.par) / 4); ++j)
+      if (64 * j + 64 <= Tokens<D, G>::kParams || lane < Tokens<D, G>::kParams - 64 * j)
+        s_par[wave][64 * j + lane] = t.par[j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes of this wave read them
+    float z[8];
+    u32x4_t vp[2];  // (scale, minimum) of the values
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        z[4 * r + i] = 0.f;
-        vs[4 * r + i] = half_lo(t.vp[r][i]);
-        vm[4 * r + i] = half_hi(t.vp[r][i]);
-      }
+      const uint32_t* par = &s_par[wave][r * 16 * (G + 1) + 4 * quad];
+      vp[r] = *reinterpret_cast<const u32x4_t*>(par + 16 * G);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        const u32x4_t kp = *reinterpret_cast<const u32x4_t*>(par + 16 * g);
         f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = g * (W / G); s < (g + 1) * (W / G); ++s) {
@@ -324,58 +455,68 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          z[4 * r + i] += fmaf(acc[i], half_lo(t.kp[r][g][i]), half_hi(t.kp[r][g][i]) * qsum[g]);
+          z[4 * r + i] = fmaf(acc[i], half_lo(kp[i]), fmaf(half_hi(kp[i]), qsum[g], g == 0 ? 0.f : z[4 * r + i]));
       }
     }
     if (32 * step + 32 > length) {  // tokens past the end: whatever the record holds must not count
+      asm volatile("");  // a branch: as selects, this is a sixth of every step's instructions
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (32 * step + 16 * (e >> 2) + 4 * quad + (e & 3) >= length) {
           z[e] = -__builtin_inff();
-          vs[e] = 0.f;
-          vm[e] = 0.f;
+          vp[e >> 2][e & 3] = 0;
         }
     }
+    __builtin_amdgcn_sched_barrier(0);  // keys, weights, values: unpacking ahead would not fit the registers
     float pe[8], pw[8];
     auto weights = [&]() {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         pe[e] = __builtin_amdgcn_exp2f(fmaf(z[e], qs, -M));
-        pw[e] = pe[e] * vs[e];
+        pw[e] = fmaf(pe[e], half_lo(vp[e >> 2][e & 3]), 0.f);  // + 0: one v_fma_mix_f32, no conversion
       }
     };
     weights();
-    float top = 0.f, top_e = 0.f;
+    float top = 0.f, sum = 0.f;
+    auto extent = [&]() {
+      top = sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      top = fmaxf(top, pw[e]);
-      top_e = fmaxf(top_e, pe[e]);
-    }
-    if (__any(top > 256.f || top_e > 0x1p60f)) {
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, pw[e]);
+        sum += pe[e];
+      }
+    };
+    extent();
+    const bool raise = __any(top > 256.f || sum > 0x1p60f);
+    float f = 1.f;
+    if (raise) {
       float m = M;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaf(z[e], qs, __log2f(fmaxf(vs[e], 0x1p-24f))));
+      for (int e = 0; e < 8; ++e)
+        m = fmaxf(m, fmaf(z[e], qs, __log2f(fmaxf(half_lo(vp[e >> 2][e & 3]), 0x1p-24f))));
       m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float f = __builtin_amdgcn_exp2f(M - m);
+      f = __builtin_amdgcn_exp2f(M - m);
       M = m;
       L *= f;
       off *= f;
-#pragma unroll
-      for (int i = 0; i < M_TILES; ++i)
-#pragma unroll
-        for (int j = 0; j < SLOTS; ++j) O[i][j] *= f;
       weights();
+      extent();
     }
     u32x4_t pf;
+    L += sum;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      L += pe[e];
-      off = fmaf(pe[e], vm[e], off);
-    }
+    for (int e = 0; e < 8; ++e) off = fmaf(pe[e], half_hi(vp[e >> 2][e & 3]), off);
 #pragma unroll
     for (int i = 0; i < 4; ++i) pf[i] = f16_pair(pw[2 * i], pw[2 * i + 1]);
 
+    if (raise) {  // apart from the above, where the compiler would keep the accumulators twice
+#pragma unroll
+      for (int i = 0; i < M_TILES; ++i)
+#pragma unroll
+        for (int j = 0; j < ACCS; ++j) O[i][j] *= f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int mt = 0; mt < M_TILES; ++mt) {
       uint32_t w[8];
@@ -397,6 +538,20 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
         }
       }
     }
+  };
+  for (int base = begin; base < last; base += ROUND * kWaves) {
+    int pages_after = pages_from(base + ROUND * kWaves);
+    for (int i = 0; i < ROUND; i += SLOTS) {
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) {
+        const int step = base + (i + j) * kWaves;
+        if (step < last) compute(slots[j], step);  // no loads in here
+        fetch(slots[j], step + SLOTS * kWaves, i + j + SLOTS);
+      }
+      if (base + (i + SLOTS) * kWaves >= last) break;
+    }
+    asm volatile("" : "+v"(pages_after));  // waited for here, where it is the oldest load, and not in the loop above
+    pages = pages_after;
   }
 
   L += __shfl_xor(L, 16, 64);
@@ -412,7 +567,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
 #pragma unroll
   for (int mt = 0; mt < M_TILES; ++mt)
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j)
+    for (int j = 0; j < ACCS; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int chunk = 16 * mt + 4 * quad + i;  // the A operand's row
@@ -425,10 +580,12 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
           channel = 8 * chunk + 2 * (j & 3) + (j >> 2);
           if (j & 1) unit = 0x1p20f;
         }
-        s_o[wave][n][channel] = O[mt][j][i] * unit;
+        sh.o[wave][n][channel] = O[mt][j][i] * unit;
       }
   __syncthreads();
-  for (int at = threadIdx.x; at < rows * D; at += 64 * kWaves) {
+  const int64_t out_row = (int64_t)seq * p.heads + h0;
+  float* slot = p.partial + (int64_t)blockIdx.x * p.plan.slot;  // [rows][D], then m and l [kRows] each
+  for (int at = threadIdx.x; at < rows * D; at += kThreads) {
     const int row = at / D, d = at % D;
     float m = s_m[0][row];
 #pragma unroll
@@ -438,42 +595,105 @@ __global__ __launch_bounds__(64 * kWaves) void kv4_attention_kernel(const Kv4Par
     for (int w = 0; w < kWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(s_m[w][row] - m);
       sum = fmaf(f, s_l[w][row], sum);
-      val = fmaf(f, s_o[w][row][d] + s_off[w][row], val);
+      val = fmaf(f, sh.o[w][row][d] + s_off[w][row], val);
     }
-    const int64_t out_row = (int64_t)seq * p.heads + h0 + row;
-    if (p.plan.splits == 1) {
-      p.out[out_row * D + d] = from_f32<DT>(length > 0 || sum != sum ? val / sum : 0.f);
+    if (share.runs == 1) {
+      p.out[out_row * D + at] = from_f32<DT>(length > 0 || sum != sum ? val / sum : 0.f);
     } else {
-      float* to = p.partial + (out_row * p.plan.splits + split) * (D + 2);
-      to[d] = val;
+      store_partial(slot + at, val);
       if (d == 0) {
-        to[D] = m;
-        to[D + 1] = sum;
+        store_partial(slot + rows * D + row, m);
+        store_partial(slot + rows * D + kRows + row, sum);
       }
     }
   }
-}
+  if (share.runs == 1) return;
 
-// Joins the runs of one query row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
-template <typename DT, int D>
-__global__ __launch_bounds__(D) void kv4_join_kernel(const Kv4Params p) {
-  const int64_t row = blockIdx.x;
-  const int seq = (int)(row / p.heads), d = threadIdx.x;
-  const int64_t capacity = (int64_t)p.table_width * p.cache.sub * 16;
-  const int64_t length = min((int64_t)max(p.lengths[seq], 0), capacity);
-  const int steps = (int)((length + 31) >> 5);
-  const int runs = max(1, min(p.plan.splits, (steps + p.plan.chunk - 1) / p.plan.chunk));
-  const float* part = p.partial + row * p.plan.splits * (D + 2);
-  float m = kLow;
-  for (int i = 0; i < runs; ++i) m = fmaxf(m, part[(int64_t)i * (D + 2) + D]);
-  float sum = 0.f, val = 0.f;
-  for (int i = 0; i < runs; ++i) {
-    const float* x = part + (int64_t)i * (D + 2);
-    const float f = __builtin_amdgcn_exp2f(x[D] - m);
-    sum = fmaf(f, x[D + 1], sum);
-    val = fmaf(f, x[d], val);
+  // as in splitk_complete: the stores have completed before the count says so
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  const int unit = seq * p.units + share.unit;
+  if (threadIdx.x == 0) s_last = atomicAdd(&p.counters[unit], 1u) == (unsigned)(share.runs - 1);
+  __syncthreads();
+  if (!s_last) return;
+  // Threads share out the columns (4 adjacent ones each) and, where there are
+  // more threads, the runs; the first loads leave before the weights are known.
+  const int runs = share.runs, columns = rows * D / 4;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      slot - (int64_t)share.run * p.plan.slot, (short)0, runs * p.plan.slot * 4, 0x00020000);
+  constexpr int BATCH = 16;
+  const int parts = max(kThreads / columns, 1), part = min((int)threadIdx.x / columns, parts);
+  f32x4_t x[BATCH];
+  auto load = [&](int column, int i0) {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      x[u] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                             rs, (min(i0 + u * parts, runs - 1) * p.plan.slot + 4 * column) * 4, 0,
+                                             kCpolSc1));
+  };
+  if (part < parts) load(threadIdx.x - part * columns, part);
+  for (int row = wave; row < rows; row += kWaves) {
+    float mi[kRuns / 64], li[kRuns / 64], m = kLow, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; ++i) {
+      const int run = lane + 64 * i, at = (run * p.plan.slot + rows * D + row) * 4;
+      mi[i] = li[i] = 0.f;
+      if (64 * i < runs) {  // past the last run: out of range, 0
+        mi[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, kCpolSc1));
+        li[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, at, 4 * kRows, kCpolSc1));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; ++i) {
+      if (lane + 64 * i >= runs) mi[i] = kLow;
+      m = fmaxf(m, mi[i]);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+#pragma unroll
+    for (int i = 0; i < kRuns / 64; ++i) {
+      const float f = __builtin_amdgcn_exp2f(mi[i] - m);
+      sum = fmaf(f, li[i], sum);
+      if (lane + 64 * i < runs) sh.join.weight[row][lane + 64 * i] = f;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) s_l[0][row] = sum;
   }
-  p.out[row * D + d] = from_f32<DT>(length > 0 || sum != sum ? val / sum : 0.f);
+  __syncthreads();
+  for (int c0 = 0; c0 < columns; c0 += kThreads) {
+    const int column = parts > 1 ? (int)threadIdx.x - part * columns : c0 + (int)threadIdx.x;
+    const bool live = part < parts && column < columns;
+    const int row = live ? column / (D / 4) : 0;
+    f32x4_t val = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      if (c0 > 0) load(column, part);
+      for (int i0 = part;;) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          if (i0 + u * parts < runs) {
+            const float f = sh.join.weight[row][i0 + u * parts];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) val[e] = fmaf(f, x[u][e], val[e]);
+          }
+        i0 += BATCH * parts;
+        if (i0 >= runs) break;
+        load(column, i0);
+      }
+    }
+    if (parts > 1) {  // one round: all columns fit the block
+      sh.join.sum[threadIdx.x] = val;
+      __syncthreads();
+      for (int i = 1; i < parts && live && part == 0; ++i) val += sh.join.sum[i * columns + column];
+    }
+    if (live && part == 0) {
+      const float inv = 1.f / s_l[0][row];
+      *reinterpret_cast<u32x2_t*>(p.out + out_row * D + 4 * column) =
+          u32x2_t{(uint32_t)from_f32<DT>(val[0] * inv) | ((uint32_t)from_f32<DT>(val[1] * inv) << 16),
+                  (uint32_t)from_f32<DT>(val[2] * inv) | ((uint32_t)from_f32<DT>(val[3] * inv) << 16)};
+    }
+  }
+  if (threadIdx.x == 0) atomicExch(&p.counters[unit], 0u);
 }
 
 // fn(DT, D, G) for the run-time dtype, head size and key groups
@@ -533,32 +753,37 @@ int launch_kv4_load(const Kv4Cache& cache, const int64_t* slots, int64_t tokens,
   });
 }
 
-Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t max_length) {
-  constexpr int64_t kBlocks = 1024;
-  const int64_t steps = max_length > 32 ? (max_length + 31) / 32 : 1;
-  const int64_t base = seqs * kv_heads * ((heads / kv_heads + kRows - 1) / kRows);
-  int64_t want = kBlocks / (base < 1 ? 1 : base);
-  want = want < 1 ? 1 : want;
-  int64_t chunk = (steps + want - 1) / want;
-  chunk = (chunk + kWaves - 1) / kWaves * kWaves;
+Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity) {
+  const int per = heads / kv_heads;
+  const int64_t units = seqs * kv_heads * ((per + kRows - 1) / kRows);
+  const int64_t steps = (capacity + 31) / 32;
   Kv4Plan plan;
-  plan.chunk = (int)chunk;
-  plan.splits = (int)((steps + chunk - 1) / chunk);
-  plan.workspace = plan.splits > 1 ? (size_t)seqs * heads * plan.splits * (head_size + 2) * sizeof(float) : 0;
+  // Eight waves per CU are in flight either way.  Up to one block per CU they
+  // are one block's, so that a long sequence is shared by half as many blocks
+  // (1 x 131072 tokens, 8 heads: 38 us with 256 blocks of 8 waves, 42 with 512 of 4);
+  // beyond, blocks of 4 waves waste less on short sequences (100 sequences of up
+  // to 300 tokens, 8 heads: 10 against 16 us).
+  plan.waves = units <= 256 ? 8 : 4;
+  plan.blocks = plan.waves == 8 ? 256 : 512;
+  plan.least = 32;  // four rounds of 8 waves: fewer cost more in the join than they save
+  plan.slot = (per < kRows ? per : kRows) * head_size + 2 * kRows;
+  // the runs beyond one per unit are at most `blocks`, and at most what the table's width allows
+  const int64_t longest = (steps + plan.least - 1) / plan.least;
+  plan.most = longest > 1 && units <= kKv4Counters ? kRuns : 1;
+  plan.grid = units;
+  if (plan.most > 1) plan.grid += units * (longest - 1) < plan.blocks ? units * (longest - 1) : plan.blocks;
+  plan.workspace =
+      plan.grid > units ? kKv4Counters * sizeof(uint32_t) + (size_t)plan.grid * plan.slot * sizeof(float) : 0;
   return plan;
 }
 
 int launch_kv4_attention(const Kv4Params& p, int dtype, hipStream_t st) {
   return dispatch_layout(dtype, p.cache.head_size, p.cache.groups, [&](auto dt, auto d, auto g) -> int {
     constexpr int D = decltype(d)::value;
-    using DT = decltype(dt);
-    const int tiles = (p.heads / p.cache.heads + kRows - 1) / kRows;
-    const int64_t blocks = (int64_t)p.seqs * p.cache.heads * tiles * p.plan.splits;
-    if (blocks > INT32_MAX || (int64_t)p.seqs * p.heads > INT32_MAX) return GRINQH_ERR_INVALID;
-    hipLaunchKernelGGL((kv4_attention_kernel<DT, D, decltype(g)::value>), dim3((uint32_t)blocks), dim3(64 * kWaves), 0,
-                       st, p);
-    if (p.plan.splits > 1)
-      hipLaunchKernelGGL((kv4_join_kernel<DT, D>), dim3((uint32_t)(p.seqs * p.heads)), dim3(D), 0, st, p);
+    if (p.plan.grid > INT32_MAX) return GRINQH_ERR_INVALID;
+    auto kernel = p.plan.waves == 8 ? kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 8>
+                                    : kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 4>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)p.plan.grid), dim3(64 * p.plan.waves), 0, st, p);
     return status();
   });
 }

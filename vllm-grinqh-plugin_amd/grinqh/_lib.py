@@ -62,7 +62,7 @@ SIGNATURES = {
     "grinqh_kv4_load": (_i32, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp]),
     "grinqh_kv4_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32, _i32, _i64]),
     "grinqh_kv4_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _i32,
-                                    _vp, _i64, ctypes.c_float, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
+                                    _vp, ctypes.c_float, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
     "grinqh_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                        _i32, _i32, _i32, ctypes.c_float, _vp, _i32, _vp]),
     "grinqh_time_next_product": (_i32, [_vp, _vp]),

@@ -24,8 +24,8 @@ from .kernel import _Workspaces, _dtype_code
 HEAD_DIMS = (64, 128, 256)
 GROUPS = (32, 64, 128, 256)
 
-# Partial results of split sequences; not the linears' workspaces, whose first
-# bytes are counters that must stay zero.
+# Counters and partial results of split sequences; the linears' workspaces have
+# counters of their own at the same place.
 _WORKSPACES = _Workspaces()
 
 
@@ -133,12 +133,10 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
-                  scale: Optional[float] = None, max_length: Optional[int] = None) -> torch.Tensor:
+                  scale: Optional[float] = None) -> torch.Tensor:
     """Attention of one query token per sequence, ``q [seqs, heads, head_dim]``, over the first ``lengths[s]`` (int32)
-    tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  ``scale`` defaults to head_dim ** -0.5.
-    ``max_length``, an upper bound of the lengths that the host knows (default: the page table's width), plans how
-    sequences are split over the GPU; longer lengths are right all the same.  A length of 0 gives zeros; a length past
-    the table or a page outside the cache NaN."""
+    tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  ``scale`` defaults to head_dim ** -0.5.  A length
+    of 0 gives zeros; a length past the table or a page outside the cache NaN."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
     dev = cache.device
     dt = _dtype_code(q.dtype)
@@ -154,15 +152,14 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         page_table = page_table.contiguous()
     lengths = _index(lengths, "lengths", torch.int32, (seqs,), dev)
     width = page_table.shape[1]
-    most = width * page if max_length is None else min(int(max_length), width * page)
     out = torch.empty((seqs, heads, d), dtype=q.dtype, device=dev)
     lib = _lib.load_library()
     stream = _stream(dev)
-    ws = _WORKSPACES.get(dev, stream, lib.grinqh_kv4_attention_workspace_bytes(seqs, heads, kv_heads, d, most))
+    ws = _WORKSPACES.get(dev, stream, lib.grinqh_kv4_attention_workspace_bytes(seqs, heads, kv_heads, d, width * page))
     qs = q.stride()
     _lib.check(lib.grinqh_kv4_attention(
         q.data_ptr(), qs[0], qs[1], seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
-        page_table.data_ptr(), page_table.stride(0), width, lengths.data_ptr(), most, _scale(scale, d), out.data_ptr(),
+        page_table.data_ptr(), page_table.stride(0), width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(),
         dt, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
         "grinqh_kv4_attention")
     return out
