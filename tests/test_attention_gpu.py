@@ -523,6 +523,11 @@ def test_prompt_strides_and_offsets():
     for q, k, v in ((x[:, 0:8], x[:, 8:12], x[:, 12:16]), (x[:, 0:16:2], flipped, x[:, 3:7]),
                     (x[:, 2:10], odd, flipped)):
         _check_prompt(ga.prompt_attention(q, k, v, _dev([0, 90, 150])), q, k, v, [0, 90, 150], [0, 90, 150], "f16")
+    for one in (x[:1, 8:12].expand(150, -1, -1), torch.zeros((150, 4, 128), dtype=torch.float16, device="cuda")):
+        _check_prompt(ga.prompt_attention(x[:, :8], one, x[:, 8:12], _dev([0, 90, 150])), x[:, :8], one, x[:, 8:12],
+                      [0, 90, 150], [0, 90, 150], "f16")
+        _check_prompt(ga.prompt_attention(x[:, :8], x[:, 8:12], one, _dev([0, 90, 150])), x[:, :8], x[:, 8:12], one,
+                      [0, 90, 150], [0, 90, 150], "f16")
     # offsets past the tensors are limited to them
     q, k, v = x[:, 0:8], x[:, 8:12], x[:, 12:16]
     out = ga.prompt_attention(q, k, v, _dev([-5, 90, 4000]))

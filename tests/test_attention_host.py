@@ -83,11 +83,11 @@ def test_c_entry_points_refuse(lib):
     assert attend(width=10000, ws=p, n=need - 1) == 3
     assert attend(width=10000, ws=bad_p, n=need) == 3
 
-    def prompt(q=p, k=p, heads=8, kv=2, d=128, rows=5, keys=5, ends=p, seqs=1, scale=0.1, out=p, dt=0):
-        return lib.grinqh_prompt_attention(q, 1024, 128, k, 256, 128, p, 256, 128, ends, p, seqs, rows, keys, heads, kv,
+    def prompt(q=p, k=p, kt=256, heads=8, kv=2, d=128, rows=5, keys=5, ends=p, seqs=1, scale=0.1, out=p, dt=0):
+        return lib.grinqh_prompt_attention(q, 1024, 128, k, kt, 128, p, 256, 128, ends, p, seqs, rows, keys, heads, kv,
                                            d, scale, out, dt, None)
 
-    for kw in ({"q": None}, {"k": bad_p}, {"heads": 3}, {"kv": 0}, {"d": 80}, {"rows": -1}, {"keys": -1},
+    for kw in ({"q": None}, {"k": bad_p}, {"kt": 0}, {"kt": 120}, {"heads": 3}, {"kv": 0}, {"d": 80}, {"rows": -1}, {"keys": -1},
                {"rows": 1 << 31}, {"ends": None}, {"seqs": -1}, {"scale": -1.0}, {"out": None}, {"dt": 9}):
         assert prompt(**kw) == 1, kw
     assert prompt(rows=0) == 0

@@ -817,7 +817,9 @@ int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, cons
       k_ends == nullptr)
     return GRINQH_ERR_INVALID;
   p.k = p.v = HeadRows{nullptr, 0, 0};
-  if (k_tokens > 0 && (!head_rows(k, k_token, k_head, &p.k) || !head_rows(v, v_token, v_head, &p.v)))
+  // keys behind a sequence's end are told from the others by their offsets
+  if (k_tokens > 0 && (!head_rows(k, k_token, k_head, &p.k) || !head_rows(v, v_token, v_head, &p.v) ||
+                       k_token < head_dim || v_token < head_dim))
     return GRINQH_ERR_INVALID;
   p.out = static_cast<uint16_t*>(out);
   p.ends = q_ends;

@@ -39,6 +39,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 constexpr int kWaves = 4;
+constexpr int kBlockRows = 32 * kWaves;
 constexpr int kKeys = 64;       // keys per tile
 constexpr float kLow = -1e30f;  // running reference before the first key (finite: -inf - -inf would be NaN)
 
@@ -52,6 +53,12 @@ __device__ __forceinline__ int wave_max(int v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
   return v;
+}
+
+// A value that all lanes agree on, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
 // One sequence's rows and keys.  Sequence `seqs` stands for the rows behind the
@@ -74,9 +81,9 @@ __device__ __forceinline__ Sequence sequence(const PromptParams& p, int s) {
 }
 
 // Block `index` of the rows' blocks, those with the most keys first: level l
-// holds the blocks whose last row sees about l * rows_per_block keys (at most one
+// holds the blocks whose last row sees about l * kBlockRows keys (at most one
 // per sequence).  Returns the sequence, or -1 past the last block.
-__device__ __forceinline__ int find_block(const PromptParams& p, int rows_per_block, int64_t index, int lane,
+__device__ __forceinline__ int find_block(const PromptParams& p, int64_t index, int lane,
                                           Sequence& found, int64_t& block) {
   const int seqs = p.seqs + 1;
   // blocks of sequence s at level >= l: their indices b + before >= l
@@ -84,8 +91,8 @@ __device__ __forceinline__ int find_block(const PromptParams& p, int rows_per_bl
     blocks = before = 0;
     if (s >= seqs) return;
     const Sequence q = sequence(p, s);
-    blocks = (int)((q.rows + rows_per_block - 1) / rows_per_block);
-    before = (int)(max(q.keys - q.rows, (int64_t)0) / rows_per_block);
+    blocks = (int)((q.rows + kBlockRows - 1) / kBlockRows);
+    before = (int)(max(q.keys - q.rows, (int64_t)0) / kBlockRows);
   };
   int my_blocks, my_before, most = 0;
   count_of(lane, my_blocks, my_before);
@@ -127,7 +134,7 @@ __device__ __forceinline__ int find_block(const PromptParams& p, int rows_per_bl
       for (int i = 0; i < (int)rank; ++i) m &= m - 1;
       const int s = s0 + __builtin_ctzll(m);
       found = sequence(p, s);
-      block = lo - (int)(max(found.keys - found.rows, (int64_t)0) / rows_per_block);
+      block = lo - (int)(max(found.keys - found.rows, (int64_t)0) / kBlockRows);
       return s;
     }
     rank -= n;
@@ -135,12 +142,16 @@ __device__ __forceinline__ int find_block(const PromptParams& p, int rows_per_bl
   return -1;
 }
 
-// Block = 4 waves x 32 * NQ query rows of one head.
-template <typename DT, int D, int NQ>
-__global__ __launch_bounds__(64 * kWaves, 1) void prompt_attention_kernel(const PromptParams p) {
-  constexpr int ROWS = kWaves * 32 * NQ, STEPS = D / 16, MT = D / 32, CHUNKS = D / 8;
-  constexpr int TILE = kKeys * D * 2;  // bytes of a tile of keys, or of values
-  extern __shared__ __align__(1024) uint8_t smem[];
+// Block = 4 waves x 32 query rows of one head.
+template <typename DT, int D>
+__global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention_kernel(const PromptParams p) {
+  constexpr int STEPS = D / 16, MT = D / 32, CHUNKS = D / 8;
+  constexpr int PER = 64 / CHUNKS;                      // keys per KiB
+  constexpr int KEY_GROUP = 1024 + (D > 128 ? 32 : 64);  // bytes from one KiB of keys to the next
+  constexpr int KEY_TILE = kKeys / PER * KEY_GROUP, VALUE_TILE = kKeys * D * 2;  // bytes
+  // separate arrays, used by name: the compiler's wait for a tile that was loaded
+  // straight into LDS is then not one for the tiles still on their way
+  __shared__ __align__(1024) uint8_t s_k0[KEY_TILE], s_k1[KEY_TILE], s_v0[VALUE_TILE], s_v1[VALUE_TILE];
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -158,180 +169,237 @@ __global__ __launch_bounds__(64 * kWaves, 1) void prompt_attention_kernel(const 
   }
   Sequence sq;
   int64_t block;
-  if (find_block(p, ROWS, index, lane, sq, block) < 0) return;
+  if (find_block(p, index, lane, sq, block) < 0) return;
+  sq = {uniform(sq.row0), uniform(sq.key0), uniform(sq.rows), uniform(sq.keys)};
+  block = uniform(block);
   const int kvh = head / (p.heads / p.kv_heads);
-  const int row0 = (int)block * ROWS + wave * 32 * NQ;  // of this wave, in the sequence
+  const int row0 = (int)block * kBlockRows + wave * 32;  // of this wave, in the sequence
   const int rows = (int)sq.rows, shift = (int)(sq.keys - sq.rows), keys = (int)sq.keys;
   // keys that the block's last row sees
-  const int block_keys = min(keys, min((int)(block + 1) * ROWS, rows) + shift);
+  const int block_keys = min(keys, min((int)(block + 1) * kBlockRows, rows) + shift);
   const int tiles = block_keys > 0 ? (block_keys + kKeys - 1) / kKeys : 0;
-  const int wave_keys = row0 < rows ? min(keys, min(row0 + 32 * NQ, rows) + shift) : 0;
+  const int wave_keys = row0 < rows ? min(keys, min(row0 + 32, rows) + shift) : 0;
 
-  // queries: row n of each 32, channels 16 s + 8 half + e
-  u32x4_t qf[NQ][STEPS];
+  // queries: row n, channels 16 s + 8 half + e
+  u32x4_t qf[STEPS];
+  {
+    const uint16_t* q = p.q.p + (sq.row0 + min(row0 + n, rows - 1)) * p.q.token + (int64_t)head * p.q.head + 8 * half;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int64_t row = sq.row0 + min(row0 + 32 * i + n, rows - 1);
-    const uint16_t* q = p.q.p + row * p.q.token + (int64_t)head * p.q.head + 8 * half;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) qf[i][s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s);
+    for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s);
   }
 
-  // LDS position of 16-byte chunk c of key r: c with bits flipped by the key, so
-  // that the 8 keys (4 key rows x 2 for the transposed read) that are read
-  // together lie in different banks
-  auto swz = [](int r) { return ((r & 3) << 2 | (r >> 2 & 3)) & (CHUNKS - 1); };
+  // LDS position of 16-byte chunk c of key r.  Loads straight into LDS put 1 KiB
+  // (PER keys) in a row, so what is read together is spread over the banks by
+  // flipping bits of c, and for the keys by a gap after every KiB as well: the
+  // keys' reads want 16 adjacent keys' chunks in 256 different bytes, the values'
+  // transposed reads 4 adjacent keys' 64 bytes.  Few bits are flipped, so that
+  // most of an address is an immediate offset.
+  auto key_swz = [](int r) { return D == 64 ? (r >> 1) & 3 : D == 128 ? r & 3 : r & 1; };
+  auto value_swz = [](int r) { return (D == 64 ? (r >> 1) & 1 : r & 3) << 2; };
+  auto key_at = [](int r) { return r / PER * KEY_GROUP + r % PER * (2 * D); };
   const uint16_t* kbase = p.k.p + sq.key0 * p.k.token + (int64_t)kvh * p.k.head;
   const uint16_t* vbase = p.v.p + sq.key0 * p.v.token + (int64_t)kvh * p.v.head;
-  auto load_tile = [&](int tile, int slot) {
-    const int k0 = tile * kKeys, live = min(kKeys, keys - k0);
-    auto one = [&](const uint16_t* base, int64_t stride, uint8_t* to) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint16_t*>(base + (int64_t)k0 * stride), (short)0, (int)(((live - 1) * stride + D) * 2),
-          0x00020000);
-      constexpr int PER = 64 / CHUNKS;  // keys per load of a wave (1 KiB)
+  // A wave loads PER keys at a time, 1 KiB; keys past the sequence's end come as
+  // zeros (behind the buffer's end, as rows are at least D apart).
+  const int load_row = wave * PER + lane / CHUNKS;
+  static_assert(kWaves * PER % 8 == 0, "the flipped bits are the same for all loads of a lane");
+  const int key_off = load_row * (int)p.k.token * 2 + (((lane % CHUNKS) ^ key_swz(load_row)) << 4);
+  const int value_off = load_row * (int)p.v.token * 2 + (((lane % CHUNKS) ^ value_swz(load_row)) << 4);
+  auto load_tile = [&](const uint16_t* base, int64_t stride, int off, int tile, uint8_t* to, int group) {
 #pragma unroll
-      for (int i = 0; i < kKeys / PER / kWaves; ++i) {
-        const int r0 = (i * kWaves + wave) * PER, r = r0 + lane / CHUNKS;
-        const int c = (lane % CHUNKS) ^ swz(r);
-        const uint32_t off = r < live ? (uint32_t)(r * stride * 2 + c * 16) : 0xFFFFFFFFu;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(to + r0 * D * 2), 16, (int)off, 0, 0, 0);
-      }
-    };
-    one(kbase, p.k.token, smem + slot * 2 * TILE);
-    one(vbase, p.v.token, smem + slot * 2 * TILE + TILE);
+    for (int i = 0; i < kKeys / PER / kWaves; ++i) {
+      const int r0 = tile * kKeys + i * kWaves * PER, live = min(kKeys, keys - r0);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(base + (int64_t)r0 * stride), (short)0,
+          live > 0 ? (int)(((live - 1) * stride + D) * 2) : 0, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(to + (i * kWaves + wave) * group), 16, off, 0, 0, 0);
+    }
   };
 
-  f32x16_t O[NQ][MT];
-  float M[NQ], sum[NQ];
+  f32x16_t O[MT];
+  float M = kLow, sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    M[i] = kLow;
-    sum[i] = 0.f;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) O[i][m] = (f32x16_t)(0.f);
-  }
+  for (int m = 0; m < MT; ++m) O[m] = (f32x16_t)(0.f);
   const float c2 = p.scale * 1.44269504088896f;
+  const int my_tiles = wave_keys > 0 ? (wave_keys + kKeys - 1) / kKeys : 0;
 
-  if (tiles > 0) load_tile(0, 0);
-  for (int tile = 0; tile < tiles; ++tile) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's share of the tile is in LDS
+  // LDS reads.  Keys: row n of key block b, channels 16 s + 8 half + e.  Values,
+  // transposed: channel 32 m + n, keys 16 t + 4 half + 0..3 and + 8.
+  const int ksw = key_swz(n), key_row = key_at(n);
+  auto read_key = [&](const uint8_t* kt, int b, int s) {
+    return *reinterpret_cast<const u32x4_t*>(kt + key_at(32 * b) + key_row + (((2 * s + half) ^ ksw) << 4));
+  };
+  const int vrow = 4 * half + ((lane & 15) >> 2), vbyte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  auto read_value = [&](const uint8_t* vt, int t, int m) {
+    u32x4_t a;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = 16 * t + 8 * u + vrow, byte = 64 * m + vbyte;
+      const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4_t)(vt + r * D * 2 + (((byte >> 4) ^ value_swz(vrow)) << 4) + (byte & 15)));
+      const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
+      a[2 * u] = y[0];
+      a[2 * u + 1] = y[1];
+    }
+    return a;
+  };
+  u32x4_t P[4];
+  // weights of two keys: pair q of key block b
+  auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], c2, -M));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], c2, -M));
+    sum += p0 + p1;
+    P[2 * b + (q >> 2)][q & 3] = pack2<DT>(p0, p1);
+  };
+  // Makes S of a tile ready for its weights: the mask where the tile reaches
+  // past a row's last key, and the reference raised where a weight would pass
+  // 2^8 (rarely after the first tiles: the accumulators are not rescaled for less).
+  auto settle = [&](f32x16_t (&S)[2], float& top, int tile) {
+    if (tile * kKeys + kKeys - 1 > row0 + shift) {
+      // last key of this tile that the row sees, less the half's 4 (compared with constants)
+      const int seen = row0 + n + shift - tile * kKeys - 4 * half;
+      top = -__builtin_inff();
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (32 * b + (e & 3) + 8 * (e >> 2) > seen) S[b][e] = -__builtin_inff();
+          top = fmaxf(top, S[b][e]);
+        }
+    }
+    if (__any(fmaf(top, c2, -M) > 8.f)) {
+      float m = fmaxf(M, top * c2);
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float f = __builtin_amdgcn_exp2f(M - m);
+      M = m;
+      sum *= f;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) O[t] *= f;
+    }
+  };
+
+  // One tile: its weights and its part of O, and the products of the next tile,
+  // slot by slot: every slot gives the matrix unit one product and the vector unit
+  // a share of the exponentials (those of keys 0..31 under the next tile's
+  // products, those of keys 32..63 under the first values'), with LDS reads AHEAD
+  // slots before their use (1: 571 us, 2: 539, 3: 533 at one sequence of 8192 rows,
+  // 32 heads of 128).
+  constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = 3;
+  auto step = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], const uint8_t* kt, const uint8_t* vt, float& top) {
+    u32x4_t f[AHEAD + 1];
+    auto read = [&](int at) {  // the A operand of slot `at`
+      f[at % (AHEAD + 1)] = at < KSLOTS ? read_key(kt, at / STEPS, at % STEPS)
+                                        : read_value(vt, (at - KSLOTS) / MT, (at - KSLOTS) % MT);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) read(k);
+    int done = 0;
+#pragma unroll
+    for (int k = 0; k < KSLOTS; ++k) {
+      const int b = k / STEPS, s = k % STEPS;
+      read(k + AHEAD);
+      N[b] = mfma32x32x16<DT>(f[k % (AHEAD + 1)], qf[s], s == 0 ? (f32x16_t)(0.f) : N[b]);
+#pragma unroll
+      for (; done < (k + 1) * 8 / KSLOTS; ++done) weigh(S, 0, done);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    done = 0;
+    int seen = 0;
+    top = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < VSLOTS; ++k) {
+      const int t = k / MT, m = k % MT;
+      if (k + AHEAD < VSLOTS) read(KSLOTS + k + AHEAD);
+      O[m] = mfma32x32x16<DT>(f[(KSLOTS + k) % (AHEAD + 1)], P[t], O[m]);
+      if (k < VSLOTS / 2) {
+#pragma unroll
+        for (; done < (k + 1) * 8 / (VSLOTS / 2); ++done) weigh(S, 1, done);
+      } else {
+#pragma unroll
+        for (; seen < (k + 1 - VSLOTS / 2) * 16 / (VSLOTS / 2); ++seen)
+          top = fmaxf(fmaxf(top, N[seen >> 3][2 * (seen & 7)]), N[seen >> 3][2 * (seen & 7) + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // Keys run one tile ahead of the values: while tile j is weighed, S of tile
+  // j + 1 is computed and the keys of j + 2 and the values of j + 1 are loaded.
+  // After the wave's last tile S is computed from whatever LDS holds, and not used:
+  // a second form of the step would cost the registers of a second O.
+  f32x16_t Sa[2], Sb[2];
+  float top;
+  if (tiles > 0) {
+    load_tile(kbase, p.k.token, key_off, 0, s_k0, KEY_GROUP);
+    load_tile(vbase, p.v.token, value_off, 0, s_v0, 1024);
+    if (tiles > 1) load_tile(kbase, p.k.token, key_off, 1, s_k1, KEY_GROUP);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's shares are in LDS
     __syncthreads();
-    if (tile + 1 < tiles) load_tile(tile + 1, (tile + 1) & 1);
-    if (tile * kKeys >= wave_keys) continue;
-    const uint8_t* kt = smem + (tile & 1) * 2 * TILE;
-    const uint8_t* vt = kt + TILE;
-    f32x16_t S[NQ][2];
+    if (my_tiles > 0) {
+      top = -__builtin_inff();
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b) {
+        Sa[b] = (f32x16_t)(0.f);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) S[i][b] = (f32x16_t)(0.f);
-      const int r = 32 * b + n;
+        for (int s = 0; s < STEPS; ++s) Sa[b] = mfma32x32x16<DT>(read_key(s_k0, b, s), qf[s], Sa[b]);
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(kt + r * D * 2 + (((2 * s + half) ^ swz(r)) << 4));
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) S[i][b] = mfma32x32x16<DT>(a, qf[i][s], S[i][b]);
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, Sa[b][e]);
       }
+      settle(Sa, top, 0);
     }
-    u32x4_t P[NQ][4];
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int seen = row0 + 32 * i + n + shift - tile * kKeys;  // last key of this tile that the row sees
-      if (tile * kKeys + kKeys - 1 > row0 + 32 * i + shift) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (32 * b + (e & 3) + 8 * (e >> 2) + 4 * half > seen) S[i][b][e] = -__builtin_inff();
-      }
-      float top = S[i][0][0];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, S[i][b][e]);
-      if (__any(fmaf(top, c2, -M[i]) > 8.f)) {
-        float m = fmaxf(M[i], top * c2);
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float f = __builtin_amdgcn_exp2f(M[i] - m);
-        M[i] = m;
-        sum[i] *= f;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) O[i][t] *= f;
-      }
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i][b][e], c2, -M[i]));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(S[i][b][e + 1], c2, -M[i]));
-          sum[i] += p0 + p1;
-          P[i][2 * b + (e >> 3)][(e & 7) >> 1] = pack2<DT>(p0, p1);
-        }
-    }
-    // values, transposed: row (channel) n, keys 16 t + 4 half + 0..3 and + 8
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        u32x4_t a;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = 16 * t + 8 * u + 4 * half + ((lane & 15) >> 2);
-          const int byte = 64 * m + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-          const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s16x4_t)(vt + r * D * 2 + (((byte >> 4) ^ swz(r)) << 4) + (byte & 15)));
-          const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
-          a[2 * u] = y[0];
-          a[2 * u + 1] = y[1];
-        }
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) O[i][m] = mfma32x32x16<DT>(a, P[i][t], O[i][m]);
-      }
   }
+  // k, v: where tile j is; v_next: the values' other slot
+  auto turn = [&](int j, uint8_t* k, uint8_t* v_next) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (j + 2 < tiles) load_tile(kbase, p.k.token, key_off, j + 2, k, KEY_GROUP);
+    if (j + 1 < tiles) load_tile(vbase, p.v.token, value_off, j + 1, v_next, 1024);
+  };
+  int j = 0;
+  for (; j + 1 < my_tiles; j += 2) {
+    turn(j, s_k0, s_v1);
+    step(Sa, Sb, s_k1, s_v0, top);
+    settle(Sb, top, j + 1);
+    turn(j + 1, s_k1, s_v0);
+    step(Sb, Sa, s_k0, s_v1, top);
+    if (j + 2 < my_tiles) settle(Sa, top, j + 2);
+  }
+  if (j < my_tiles) {
+    turn(j, s_k0, s_v1);
+    step(Sa, Sb, s_k1, s_v0, top);
+    ++j;
+  }
+  for (; j < tiles; ++j) turn(j, (j & 1) ? s_k1 : s_k0, (j & 1) ? s_v0 : s_v1);  // the other waves' tiles
 
+  const float l = sum + __shfl_xor(sum, 32, 64);
+  const int row = row0 + n;
+  if (row >= rows) return;
+  const float inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees no key gives zeros
+  uint16_t* o = p.out + ((sq.row0 + row) * p.heads + head) * D + 4 * half;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const float l = sum[i] + __shfl_xor(sum[i], 32, 64);
-    const int row = row0 + 32 * i + n;
-    if (row >= rows) continue;
-    const float inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees no key gives zeros
-    uint16_t* o = p.out + ((sq.row0 + row) * p.heads + head) * D + 4 * half;
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) =
-            u32x2_t{pack2<DT>(O[i][m][e] * inv, O[i][m][e + 1] * inv),
-                    pack2<DT>(O[i][m][e + 2] * inv, O[i][m][e + 3] * inv)};
-  }
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) = u32x2_t{
+          pack2<DT>(O[m][e] * inv, O[m][e + 1] * inv), pack2<DT>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
 }
 
 }  // namespace
 
 int launch_prompt_attention(const PromptParams& p, int dtype, hipStream_t st) {
-  auto go = [&](auto dt, auto d, auto nq) -> int {
-    constexpr int D = decltype(d)::value, NQ = decltype(nq)::value, ROWS = kWaves * 32 * NQ;
-    auto kernel = prompt_attention_kernel<decltype(dt), D, NQ>;
-    const int lds = 4 * kKeys * D * 2;
-    const int64_t blocks = ((p.q_tokens + ROWS - 1) / ROWS + p.seqs) * p.heads;
+  auto go = [&](auto kernel) -> int {
+    const int64_t blocks = ((p.q_tokens + kBlockRows - 1) / kBlockRows + p.seqs) * p.heads;
     if (blocks > INT32_MAX) return GRINQH_ERR_INVALID;
-    if (lds > 64 * 1024)
-      if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
-          hipSuccess)
-        return GRINQH_ERR_HIP;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * kWaves), lds, st, p);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * kWaves), 0, st, p);
     return hipGetLastError() == hipSuccess ? GRINQH_OK : GRINQH_ERR_HIP;
   };
-  auto sized = [&](auto dt) -> int {
-    switch (p.head_size) {
-      case 64: return go(dt, std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-      case 128: return go(dt, std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
-      case 256: return go(dt, std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
-    }
-    return GRINQH_ERR_INVALID;
-  };
-  return dtype == GRINQH_DTYPE_BF16 ? sized(BF16{}) : sized(F16{});
+  const bool bf16 = dtype == GRINQH_DTYPE_BF16;
+  switch (p.head_size) {
+    case 64: return bf16 ? go(prompt_attention_kernel<BF16, 64>) : go(prompt_attention_kernel<F16, 64>);
+    case 128: return bf16 ? go(prompt_attention_kernel<BF16, 128>) : go(prompt_attention_kernel<F16, 128>);
+    case 256: return bf16 ? go(prompt_attention_kernel<BF16, 256>) : go(prompt_attention_kernel<F16, 256>);
+  }
+  return GRINQH_ERR_INVALID;
 }
 
 }  // namespace grinqh

@@ -179,6 +179,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
     v = _rows(v, "v", dev, q.dtype)
     tokens, heads, d = q.shape
     keys, kv_heads, dk = k.shape
+    if k.stride(0) < dk:  # broadcast or overlapping rows
+        k = k.contiguous()
+    if v.stride(0) < dk:
+        v = v.contiguous()
     if d not in HEAD_DIMS or dk != d or v.shape != k.shape or kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"GRINQH: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit: head_dim "
                          f"must be one of {HEAD_DIMS}, the heads a multiple of the key/value heads")
