@@ -44,36 +44,50 @@ __device__ __forceinline__ float half_hi(uint32_t w) { return f16_bits_to_f32((u
 
 // ---------------------------------------------------------------- store, load
 
+// The value of the lane that DPP control `CTRL` names.
+template <int CTRL>
+__device__ __forceinline__ float lane_value(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// op over WIDTH adjacent lanes, in all of them: neighbours within 4 by quad
+// permutes, then the mirrored half of 8 and of 16 (any lane of the other half
+// will do), then the other 16 of 32.
+template <int WIDTH, typename F>
+__device__ __forceinline__ float group_reduce(float v, F&& op) {
+  v = op(v, lane_value<0xB1>(v));
+  v = op(v, lane_value<0x4E>(v));
+  if constexpr (WIDTH >= 8) v = op(v, lane_value<0x141>(v));
+  if constexpr (WIDTH >= 16) v = op(v, lane_value<0x140>(v));
+  if constexpr (WIDTH >= 32) v = op(v, __shfl_xor(v, 16, 64));
+  return v;
+}
+
 // Codes and (scale, minimum) of one lane's 8 channels; the WIDTH adjacent lanes
 // of a group share the parameters.  A NaN becomes +inf in the maximum, which
-// no finite input reaches, and makes the group's parameters NaN.
+// the limit keeps finite inputs from, and makes the group's parameters NaN.
+// Channels past the limit need no limiting of their own: their codes do it.
+// VALU bound for long prompts (16 values per lane, some ten operations each).
 template <typename DT, int WIDTH>
 __device__ __forceinline__ uint32_t quantize8(const u32x4_t& in, uint32_t& params) {
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = to_f32<DT>((uint16_t)(in[e >> 1] >> (16 * (e & 1))));
-  bool nan = false;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    nan = nan || x[e] != x[e];
-    x[e] = fminf(fmaxf(x[e], -kLimit), kLimit);
-  }
   float mn = x[0], mx = x[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) {
     mn = fminf(mn, x[e]);
-    mx = fmaxf(mx, x[e]);
+    mx = __builtin_elementwise_maximum(mx, x[e]);  // NaN if one is
   }
-  if (nan) mx = __builtin_inff();
-#pragma unroll
-  for (int o = 1; o < WIDTH; o <<= 1) {
-    mn = fminf(mn, __shfl_xor(mn, o, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  }
+  mn = fmaxf(mn, -kLimit);
+  mx = mx != mx ? __builtin_inff() : fminf(mx, kLimit);
+  mn = group_reduce<WIDTH>(mn, [](float a, float b) { return fminf(a, b); });
+  mx = group_reduce<WIDTH>(mx, [](float a, float b) { return fmaxf(a, b); });
   if (mx > kLimit) {
     params = 0x7E007E00u;  // NaN, NaN
     return 0;
   }
+  mn = fminf(mn, kLimit);   // where every channel is past the limit
+  mx = fmaxf(mx, -kLimit);
   const uint16_t mh = f32_to_f16_bits(mn + 0.f);  // zeros are kept as +0, whichever zero came first
   const float m = f16_bits_to_f32(mh);
   const uint16_t sh = f32_to_f16_bits((mx - m) * (1.f / 15.f) + 0.f);

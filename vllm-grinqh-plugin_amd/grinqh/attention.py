@@ -14,6 +14,7 @@ attention to vLLM.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -58,62 +59,66 @@ def _cache_layout(cache: torch.Tensor) -> Tuple[int, int, int, int, int]:
     """(pages, kv_heads, page_size, head_dim, group) of a cache tensor"""
     if not cache.is_cuda:
         raise ValueError("GRINQH: the cache must be on a HIP device; there is no CPU path")
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[3] not in _LAYOUTS or not cache.is_contiguous():
+    shape = cache.shape
+    layout = _LAYOUTS.get(shape[3]) if len(shape) == 4 else None
+    if layout is None or cache.dtype is not torch.uint8 or not cache.is_contiguous():
         raise ValueError("GRINQH: a cache is a contiguous uint8 tensor [pages, kv_heads, page_size / 16, record] "
-                         f"(kv4_cache), got {cache.dtype} {tuple(cache.shape)}")
-    pages, heads, sub, record = cache.shape
-    return (pages, heads, 16 * sub, *_LAYOUTS[record])
+                         f"(kv4_cache), got {cache.dtype} {tuple(shape)}")
+    return shape[0], shape[1], 16 * shape[2], layout[0], layout[1]
 
 
-def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """x [tokens, heads, head_dim] as the kernels read it: 16-byte aligned rows, token and head distances multiples
-    of 8; copied where it is not."""
-    if x.device != device or not x.is_cuda:
-        raise ValueError(f"GRINQH: {name} must be on the HIP device of the other arguments, got {x.device}")
-    if x.dim() != 3:
-        raise ValueError(f"GRINQH: {name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
-    if dtype is not None and x.dtype != dtype:
-        raise ValueError(f"GRINQH: {name} must be {dtype}, got {x.dtype}")
+def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> Tuple[torch.Tensor, int, int]:
+    """x [tokens, heads, head_dim] as the kernels read it (16-byte aligned rows, distances multiples of 8; copied
+    where it is not), and its token and head distances"""
+    if x.device != device or x.dtype is not dtype:
+        raise ValueError(f"GRINQH: {name} must be {dtype} on {device}, got {x.dtype} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"GRINQH: {name} requires a gradient; the attention operators have no backward pass")
-    t, h, c = x.stride()
-    if c != 1 or t % 8 or h % 8 or not 0 <= t <= 1 << 23 or not 0 <= h <= 1 << 23 or x.data_ptr() % 16:
+    stride = x.stride()
+    if len(stride) != 3:
+        raise ValueError(f"GRINQH: {name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
+    t, h, c = stride
+    if c != 1 or t % 8 or h % 8 or t > 1 << 23 or h > 1 << 23 or x.data_ptr() % 16:
         x = x.contiguous()
-    return x
+        t, h, c = x.stride()
+    return x, t, h
 
 
-def _index(x: torch.Tensor, name: str, dtype: torch.dtype, shape: Tuple[int, ...], device: torch.device) -> torch.Tensor:
-    if x.device != device or x.dtype != dtype or tuple(x.shape) != shape:
-        raise ValueError(f"GRINQH: {name} must be {dtype} {list(shape)} on {device}, got {x.dtype} {list(x.shape)} on "
+def _index(x: torch.Tensor, name: str, dtype: torch.dtype, n: int, device: torch.device) -> torch.Tensor:
+    if x.device != device or x.dtype is not dtype or x.dim() != 1 or x.shape[0] != n:
+        raise ValueError(f"GRINQH: {name} must be {dtype} [{n}] on {device}, got {x.dtype} {list(x.shape)} on "
                          f"{x.device}")
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_stream = torch._C._cuda_getCurrentRawStream  # current_stream() without its wrapper object
 
 
 def _scale(scale: Optional[float], head_dim: int) -> float:
     return head_dim ** -0.5 if scale is None else float(scale)
 
 
+@lru_cache(maxsize=1024)
+def _workspace_bytes(seqs: int, heads: int, kv_heads: int, head_dim: int, capacity: int) -> int:
+    return _lib.load_library().grinqh_kv4_attention_workspace_bytes(seqs, heads, kv_heads, head_dim, capacity)
+
+
 def kv4_store(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write keys and values ``[tokens, kv_heads, head_dim]`` at ``slots`` (int64 ``[tokens]``: page * page_size +
     place).  Slots outside the cache (-1: padding) are skipped; no two tokens may have the same slot."""
     pages, heads, page, d, group = _cache_layout(cache)
-    dev = cache.device
-    dt = _dtype_code(k.dtype)
-    k = _rows(k, "k", dev)
-    v = _rows(v, "v", dev, k.dtype)
+    dev, dtype = cache.device, k.dtype
+    dt = _dtype_code(dtype)
+    k, k_token, k_head = _rows(k, "k", dev, dtype)
+    v, v_token, v_head = _rows(v, "v", dev, dtype)
     n = k.shape[0]
     if k.shape != (n, heads, d) or v.shape != k.shape:
         raise ValueError(f"GRINQH: k and v must be [tokens, {heads}, {d}] for this cache, got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
-    slots = _index(slots, "slots", torch.int64, (n,), dev)
-    ks, vs = k.stride(), v.stride()
+    slots = _index(slots, "slots", torch.int64, n, dev)
     _lib.check(_lib.load_library().grinqh_kv4_store(
-        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], slots.data_ptr(), n, cache.data_ptr(), pages, heads,
-        page, d, group, dt, _stream(dev)), "grinqh_kv4_store")
+        k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, slots.data_ptr(), n, cache.data_ptr(), pages,
+        heads, page, d, group, dt, _stream(dev.index)), "grinqh_kv4_store")
 
 
 def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
@@ -122,13 +127,13 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     pages, heads, page, d, group = _cache_layout(cache)
     dev = cache.device
     dt = _dtype_code(dtype)
-    n = slots.shape[0]
-    slots = _index(slots, "slots", torch.int64, (n,), dev)
+    n = slots.numel()
+    slots = _index(slots, "slots", torch.int64, n, dev)
     k = torch.empty((n, heads, d), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     _lib.check(_lib.load_library().grinqh_kv4_load(
         cache.data_ptr(), pages, heads, page, d, group, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt,
-        _stream(dev)), "grinqh_kv4_load")
+        _stream(dev.index)), "grinqh_kv4_load")
     return k, v
 
 
@@ -138,29 +143,30 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  ``scale`` defaults to head_dim ** -0.5.  A length
     of 0 gives zeros; a length past the table or a page outside the cache NaN."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
-    dev = cache.device
-    dt = _dtype_code(q.dtype)
-    q = _rows(q, "q", dev)
+    dev, dtype = cache.device, q.dtype
+    dt = _dtype_code(dtype)
+    q, q_token, q_head = _rows(q, "q", dev, dtype)
     seqs, heads, dq = q.shape
     if dq != d or heads % kv_heads:
         raise ValueError(f"GRINQH: q {tuple(q.shape)} does not match a cache of {kv_heads} heads of {d} channels")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev or \
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.device != dev or \
             page_table.shape[0] != seqs:
         raise ValueError(f"GRINQH: page_table must be torch.int32 [{seqs}, width] on {dev}, got {page_table.dtype} "
                          f"{list(page_table.shape)} on {page_table.device}")
-    if page_table.stride(1) != 1:
+    table_stride, one = page_table.stride()
+    if one != 1:
         page_table = page_table.contiguous()
-    lengths = _index(lengths, "lengths", torch.int32, (seqs,), dev)
+        table_stride = page_table.stride(0)
+    lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
     width = page_table.shape[1]
-    out = torch.empty((seqs, heads, d), dtype=q.dtype, device=dev)
-    lib = _lib.load_library()
-    stream = _stream(dev)
-    ws = _WORKSPACES.get(dev, stream, lib.grinqh_kv4_attention_workspace_bytes(seqs, heads, kv_heads, d, width * page))
-    qs = q.stride()
-    _lib.check(lib.grinqh_kv4_attention(
-        q.data_ptr(), qs[0], qs[1], seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
-        page_table.data_ptr(), page_table.stride(0), width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(),
-        dt, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
+    out = torch.empty((seqs, heads, d), dtype=dtype, device=dev)
+    stream = _stream(dev.index)
+    nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
+    ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
+    _lib.check(_lib.load_library().grinqh_kv4_attention(
+        q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
+        page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
+        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
         "grinqh_kv4_attention")
     return out
 
@@ -172,34 +178,35 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
     ``key_ends[s] .. key_ends[s + 1] - 1`` (default: as its rows); its last row sees all its keys, the row before one
     fewer, and so on.  Rows that see no key, or lie behind the last sequence, give zeros.  ``scale`` defaults to
     head_dim ** -0.5."""
-    dev = q.device
-    dt = _dtype_code(q.dtype)
-    q = _rows(q, "q", dev)
-    k = _rows(k, "k", dev, q.dtype)
-    v = _rows(v, "v", dev, q.dtype)
+    dev, dtype = q.device, q.dtype
+    if not q.is_cuda:
+        raise ValueError(f"GRINQH: q must be on a HIP device (got {dev}); there is no CPU path")
+    dt = _dtype_code(dtype)
+    q, q_token, q_head = _rows(q, "q", dev, dtype)
+    k, k_token, k_head = _rows(k, "k", dev, dtype)
+    v, v_token, v_head = _rows(v, "v", dev, dtype)
     tokens, heads, d = q.shape
     keys, kv_heads, dk = k.shape
-    if k.stride(0) < dk:  # broadcast or overlapping rows
-        k = k.contiguous()
-    if v.stride(0) < dk:
-        v = v.contiguous()
+    if k_token < dk:  # broadcast or overlapping rows
+        k, k_token, k_head = _rows(k.contiguous(), "k", dev, dtype)
+    if v_token < dk:
+        v, v_token, v_head = _rows(v.contiguous(), "v", dev, dtype)
     if d not in HEAD_DIMS or dk != d or v.shape != k.shape or kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"GRINQH: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit: head_dim "
                          f"must be one of {HEAD_DIMS}, the heads a multiple of the key/value heads")
-    if ends.dim() != 1 or ends.shape[0] == 0:
+    seqs = ends.numel() - 1
+    if seqs < 0:
         raise ValueError(f"GRINQH: ends must be int32 [seqs + 1], got {list(ends.shape)}")
-    seqs = ends.shape[0] - 1
-    ends = _index(ends, "ends", torch.int32, (seqs + 1,), dev)
+    ends = _index(ends, "ends", torch.int32, seqs + 1, dev)
     if key_ends is None:
         if keys != tokens:
             raise ValueError(f"GRINQH: {keys} keys for {tokens} rows need key_ends")
         key_ends = ends
     else:
-        key_ends = _index(key_ends, "key_ends", torch.int32, (seqs + 1,), dev)
-    out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
+        key_ends = _index(key_ends, "key_ends", torch.int32, seqs + 1, dev)
+    out = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
     _lib.check(_lib.load_library().grinqh_prompt_attention(
-        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], ends.data_ptr(),
+        q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, ends.data_ptr(),
         key_ends.data_ptr(), seqs, tokens, keys, heads, kv_heads, d, _scale(scale, d), out.data_ptr(), dt,
-        _stream(dev)), "grinqh_prompt_attention")
+        _stream(dev.index)), "grinqh_prompt_attention")
     return out
