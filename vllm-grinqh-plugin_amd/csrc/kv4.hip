@@ -26,6 +26,7 @@
 #include "attention_launch.h"
 #include "grinqh_common.h"
 #include "splitk_complete.h"
+#include "wave_scan.h"
 
 namespace grinqh {
 
@@ -174,24 +175,6 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Cache cache, const int
 constexpr int kRows = 16;       // query heads of one key/value head per block
 constexpr int kRuns = 256;      // most blocks that share one sequence and head
 constexpr float kLow = -1e30f;  // running reference before the first token (finite: -inf - -inf would be NaN)
-
-// Inclusive sum over the lanes of a wave (row shifts, then the rows' totals).
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  auto step = [&](auto ctrl, auto rows) {
-    const int x = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value,
-                                              decltype(rows)::value, 0xf, false);
-    v += __builtin_bit_cast(T, x);
-  };
-  using I = std::integral_constant<int, 0xf>;
-  step(std::integral_constant<int, 0x111>{}, I{});
-  step(std::integral_constant<int, 0x112>{}, I{});
-  step(std::integral_constant<int, 0x114>{}, I{});
-  step(std::integral_constant<int, 0x118>{}, I{});
-  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
-  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
-  return v;
-}
 
 // Which run of 32-token steps a block takes.
 struct Share {
@@ -521,8 +504,16 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
     L += sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) off = fmaf(pe[e], half_hi(vp[e >> 2][e & 3]), off);
+    // The weights' rounding to fp16 would be multiplied by codes of 7.5 on
+    // average, where the values themselves are near zero: what it takes from the
+    // codes' middle is added back (fp16 results 4.8e-4 -> 1.7e-4 off beside their own
+    // rounding of 2.1e-4).
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pf[i] = f16_pair(pw[2 * i], pw[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      pf[i] = f16_pair(pw[2 * i], pw[2 * i + 1]);
+      off = fmaf(7.5f, fmaf(half_lo(pf[i]), -1.f, pw[2 * i]), off);
+      off = fmaf(7.5f, fmaf(half_hi(pf[i]), -1.f, pw[2 * i + 1]), off);
+    }
 
     if (raise) {  // apart from the above, where the compiler would keep the accumulators twice
 #pragma unroll

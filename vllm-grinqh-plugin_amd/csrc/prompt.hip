@@ -10,6 +10,7 @@
 
 #include "attention_launch.h"
 #include "grinqh_common.h"
+#include "wave_scan.h"
 
 namespace grinqh {
 
@@ -42,18 +43,6 @@ constexpr int kWaves = 4;
 constexpr int kBlockRows = 32 * kWaves;
 constexpr int kKeys = 64;       // keys per tile
 constexpr float kLow = -1e30f;  // running reference before the first key (finite: -inf - -inf would be NaN)
-
-// Sum over the wave, in every lane.
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
-}
 
 // A value that all lanes agree on, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -94,7 +83,7 @@ __device__ __forceinline__ int find_block(const PromptParams& p, int64_t index, 
     blocks = (int)((q.rows + kBlockRows - 1) / kBlockRows);
     before = (int)(max(q.keys - q.rows, (int64_t)0) / kBlockRows);
   };
-  int my_blocks, my_before, most = 0;
+  int my_blocks, my_before;
   count_of(lane, my_blocks, my_before);
   auto at_least = [&](int level) {
     int sum = 0;
@@ -105,14 +94,12 @@ __device__ __forceinline__ int find_block(const PromptParams& p, int64_t index, 
     }
     return wave_sum(sum);
   };
-  for (int s = lane; s < seqs; s += 64) {
-    int blocks = my_blocks, before = my_before;
-    if (s >= 64) count_of(s, blocks, before);
-    if (blocks > 0) most = max(most, blocks + before);
-  }
-  most = wave_max(most);
   if (index >= at_least(0)) return -1;
-  int lo = 0, hi = most;  // at_least(lo) > index >= at_least(hi)
+  int lo = 0, hi = 1;  // at_least(lo) > index >= at_least(hi)
+  while (at_least(hi) > index) {
+    lo = hi;
+    hi *= 2;
+  }
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (at_least(mid) > index)
