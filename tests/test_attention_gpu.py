@@ -270,7 +270,7 @@ def test_decode_split_lengths(lens, hkv, per):
             _check_decode(ga.kv4_attention(q, cache, tab, lengths), q, kv, 128, "bf16")
 
 
-@pytest.mark.parametrize("seqs", [63, 64, 65, 130, 700])
+@pytest.mark.parametrize("seqs", [63, 64, 65, 130, 700, 1024, 1025])
 def test_decode_many_sequences(seqs):
     from grinqh import attention as ga
     rng = np.random.default_rng(seqs)

@@ -101,4 +101,5 @@ def test_workspace_query(lib):
     assert q(1, 32, 8, 128, 131072) == counters + (8 + 256) * (4 * 128 + 32) * 4
     assert q(1, 64, 1, 64, 131072) == counters + (4 + 256) * (16 * 64 + 32) * 4   # 4 tiles of 16 query heads
     assert q(5000, 32, 8, 128, 131072) == 0     # more units than counters: none is shared
+    assert q(1024, 4, 1, 128, 131072) > 0 and q(1025, 4, 1, 128, 131072) == 0   # more sequences than a plan covers
     assert q(0, 32, 8, 128, 100) == 0 and q(1, 5, 2, 128, 100) == 0 and q(1, 4, 2, 128, 0) == 0

@@ -67,7 +67,9 @@ __device__ __forceinline__ float group_reduce(float v, F&& op) {
 // of a group share the parameters.  A NaN becomes +inf in the maximum, which
 // the limit keeps finite inputs from, and makes the group's parameters NaN.
 // Channels past the limit need no limiting of their own: their codes do it.
-// VALU bound for long prompts (16 values per lane, some ten operations each).
+// VALU bound for long prompts (16 values per lane, some ten operations each):
+// 8192 tokens of 8 heads of 128 channels take 12.7 us to store (43 MB, 3.4 TB/s)
+// and 8.1 to load (5.3 TB/s).
 template <typename DT, int WIDTH>
 __device__ __forceinline__ uint32_t quantize8(const u32x4_t& in, uint32_t& params) {
   float x[8];
@@ -173,6 +175,7 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Cache cache, const int
 // ---------------------------------------------------------------- attention, one token per sequence
 
 constexpr int kRows = 16;       // query heads of one key/value head per block
+constexpr int kGroup = 16;     // sequences a lane looks at: plans cover 64 of these
 constexpr int kRuns = 256;      // most blocks that share one sequence and head
 constexpr float kLow = -1e30f;  // running reference before the first token (finite: -inf - -inf would be NaN)
 
@@ -194,8 +197,10 @@ __device__ __forceinline__ int length_of(const Kv4Params& p, int seq, bool& bad)
 // Every block plans by itself from the lengths, which only the device knows:
 // the steps of all sequences and heads shared out over plan.blocks, in runs of
 // at least plan.least steps that never leave their sequence, all runs of a
-// sequence alike.  A lane sums up seqs / 64 sequences, a scan over the lanes
-// finds the block's.  False: more blocks than runs.
+// sequence alike.  A lane looks at seqs / 64 sequences (at most kGroup: with more
+// there are blocks enough, and a plan would take longer), a scan over the lanes
+// finds the block's.  Where no sequence can be shared (plan.most == 1) a block
+// is a unit.  False: more blocks than runs.
 __device__ __forceinline__ bool find_share(const Kv4Params& p, int id, int lane, Share& s) {
   if (p.plan.most == 1) {
     s.seq = id / p.units;
@@ -207,39 +212,44 @@ __device__ __forceinline__ bool find_share(const Kv4Params& p, int id, int lane,
     return true;
   }
   const int group = (p.seqs + 63) >> 6, s0 = lane * group;
+  int mine[kGroup];  // lengths of the lane's sequences
   bool bad = false;
-  const int mine = lane < p.seqs ? length_of(p, lane, bad) : 0;  // all there is with up to 64 sequences
-  const uint64_t bads = __ballot(bad);
-  auto steps_of = [&](int i) {  // of the lane's i-th sequence
+  mine[0] = s0 < p.seqs ? length_of(p, s0, bad) : 0;
+#pragma unroll
+  for (int i = 1; i < kGroup; ++i) {
     bool b;
-    return ((group == 1 ? mine : length_of(p, s0 + i, b)) + 31) >> 5;
-  };
+    mine[i] = group > 1 && i < group && s0 + i < p.seqs ? length_of(p, s0 + i, b) : 0;
+  }
   float steps = 0.f;
-  for (int i = 0; i < group; ++i)
-    if (s0 + i < p.seqs) steps += (float)steps_of(i);
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) steps += (float)((mine[i] + 31) >> 5);
   const float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(steps)), 63));
   const int chunk = max(p.plan.least, (int)ceilf(fminf(total * (float)p.units / (float)p.plan.blocks, 0x1p26f)));
-  auto runs_of = [&](int n) { return min(max((n + chunk - 1) / chunk, 1), p.plan.most); };
+  auto runs_of = [&](int length) { return min(max((((length + 31) >> 5) + chunk - 1) / chunk, 1), p.plan.most); };
   int runs = 0;
-  for (int i = 0; i < group; ++i)
-    if (s0 + i < p.seqs) runs += runs_of(steps_of(i)) * p.units;
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i)
+    if (i < group && s0 + i < p.seqs) runs += runs_of(mine[i]) * p.units;
   const int upto = wave_scan(runs);
   const uint64_t after = __ballot(upto > id);
   if (after == 0) return false;
   const int owner = __builtin_ctzll(after);
   int rest = id - __builtin_amdgcn_readlane(upto - runs, owner);
-  int seq = owner * group, k = 1;
-  for (;; ++seq) {
-    if (group == 1) {
-      s.length = __builtin_amdgcn_readlane(mine, seq);
-      s.bad = (bads >> seq) & 1;
+  int seq = owner * group, k = 0;
+  s.length = 0;
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    if (i >= group || k > 0) break;
+    s.length = __builtin_amdgcn_readlane(mine[i], owner);
+    const int r = runs_of(s.length);
+    if (rest < r * p.units) {
+      k = r;
     } else {
-      s.length = __builtin_amdgcn_readfirstlane(length_of(p, seq, s.bad));
+      rest -= r * p.units;
+      ++seq;
     }
-    k = runs_of((s.length + 31) >> 5);
-    if (rest < k * p.units) break;
-    rest -= k * p.units;
   }
+  s.bad = group == 1 ? (__ballot(bad) >> owner) & 1 : p.lengths[seq] > s.length;  // limited, hence past the table
   const int n = (s.length + 31) >> 5, per = (n + k - 1) / k;
   s.seq = seq;
   s.runs = k;
@@ -301,13 +311,20 @@ __device__ __forceinline__ void load_tokens(Tokens<D, G>& t, const uint8_t* __re
 // each leaves its result in the workspace and the one that arrives last joins
 // them, in their order.
 //
+// Bound by HBM for long contexts: 64 sequences of 8192 tokens, 32 query and 8
+// key/value heads of 128 (570 MB) take 103 us, 5.5 TB/s; a kernel that only reads
+// the same pages takes 95, the difference is the blocks' start and end.  One
+// sequence of 131072 tokens: 37 us (147 MB, 4.0 TB/s with planning and joining).
+// Short ones are latency: lengths, pages, tokens, one after the other, 7-10 us.
+//
 // S^T = K Q^T leaves a lane with one query row and 8 of the 32 tokens, which
 // is the B operand of O^T = V^T P^T: nothing crosses lanes in the loop.  With
 // value = m + s c:  o = sum_t (p_t s_t) c_t + sum_t p_t m_t, so P carries the
 // value scale and the minimum is one sum per row.
 //
 // The exponent's reference M is raised only when a weight p s passes 2^8
-// (checked for all lanes at once), so the accumulators are rarely rescaled;
+// (checked for all lanes at once; as a branch apart from the weights, or the
+// compiler keeps the accumulators twice), so the accumulators are rarely rescaled;
 // M includes the value scale, which keeps the fp16 weights in range whatever
 // the values' size.  Queries are brought to 2^13 <= max < 2^14 by a power of two
 // (exact), so fp16 holds them for both types and the nibbles that come out
@@ -774,7 +791,7 @@ Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t c
   plan.slot = (per < kRows ? per : kRows) * head_size + 2 * kRows;
   // the runs beyond one per unit are at most `blocks`, and at most what the table's width allows
   const int64_t longest = (steps + plan.least - 1) / plan.least;
-  plan.most = longest > 1 && units <= kKv4Counters ? kRuns : 1;
+  plan.most = longest > 1 && units <= kKv4Counters && seqs <= 64 * kGroup ? kRuns : 1;
   plan.grid = units;
   if (plan.most > 1) plan.grid += units * (longest - 1) < plan.blocks ? units * (longest - 1) : plan.blocks;
   plan.workspace =
