@@ -222,18 +222,24 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
 
   // LDS reads.  Keys: row n of key block b, channels 16 s + 8 half + e.  Values,
   // transposed: channel 32 m + n, keys 16 t + 4 half + 0..3 and + 8.
-  const int ksw = key_swz(n), key_row = key_at(n);
+  // The flipped bits make two bases (four for the values), the rest are offsets.
+  int key_base[2], value_base[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) key_base[i] = key_at(n) + (((2 * i + half) ^ key_swz(n)) << 4);
+  const int vrow = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    value_base[i] = vrow * D * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ value_swz(vrow)) << 4) +
+                    8 * (lane & 1);
   auto read_key = [&](const uint8_t* kt, int b, int s) {
-    return *reinterpret_cast<const u32x4_t*>(kt + key_at(32 * b) + key_row + (((2 * s + half) ^ ksw) << 4));
+    return *reinterpret_cast<const u32x4_t*>(kt + key_base[s & 1] + key_at(32 * b) + 64 * (s >> 1));
   };
-  const int vrow = 4 * half + ((lane & 15) >> 2), vbyte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
   auto read_value = [&](const uint8_t* vt, int t, int m) {
     u32x4_t a;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int r = 16 * t + 8 * u + vrow, byte = 64 * m + vbyte;
       const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s16x4_t)(vt + r * D * 2 + (((byte >> 4) ^ value_swz(vrow)) << 4) + (byte & 15)));
+          (lds_s16x4_t)(vt + value_base[m & 3] + (16 * t + 8 * u) * D * 2 + 256 * (m >> 2)));
       const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
       a[2 * u] = y[0];
       a[2 * u + 1] = y[1];
