@@ -315,7 +315,7 @@ __device__ __forceinline__ void load_tokens(Tokens<D, G>& t, const uint8_t* __re
 // key/value heads of 128 (570 MB) take 103 us, 5.5 TB/s; a kernel that only reads
 // the same pages takes 95, the difference is the blocks' start and end.  One
 // sequence of 131072 tokens: 37 us (147 MB, 4.0 TB/s with planning and joining).
-// Short ones are latency: lengths, pages, tokens, one after the other, 7-10 us.
+// Short ones are latency: lengths, pages, tokens, one after the other, 8-11 us.
 //
 // S^T = K Q^T leaves a lane with one query row and 8 of the 32 tokens, which
 // is the B operand of O^T = V^T P^T: nothing crosses lanes in the loop.  With

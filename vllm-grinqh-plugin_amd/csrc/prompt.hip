@@ -13,10 +13,10 @@
 // operations, 32 of them v_exp_f32 (8 cycles with two waves per SIMD, 16 with
 // one).  One wave per SIMD issues a VALU operation every 6 cycles at most, two
 // every 4-5 (measured), so a wave has 32 rows and a SIMD two waves (64 rows and one
-// wave per SIMD also spilled); the LDS reads of 32 rows take half of the
-// products' time.  One sequence of 8192 rows, 32 heads: 534 us, 1030 TFLOP/s,
-// where a library product of 8192^3 reaches 1400.  Heads of 256 channels need 480
-// registers, one wave per SIMD: 460 TFLOP/s.
+// wave per SIMD would read LDS half as often, but took 826 us: accumulators moved
+// between the register files).  One sequence of 8192 rows, 32 heads: 528 us, 1040
+// TFLOP/s, where a library product of 8192^3 reaches 1400.  Heads of 256 channels
+// need 440 registers, one wave per SIMD: 490 TFLOP/s.
 #include <type_traits>
 
 #include "attention_launch.h"
