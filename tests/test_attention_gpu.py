@@ -435,8 +435,8 @@ def test_prompt(dtype, d, hq, hkv):
     rng = np.random.default_rng(d + hq)
     lens = [1, 0, 63, 64, 65, 2, 127, 129, 0, 300]
     ends = _ends(lens)
-    x = _randn(rng, ends[-1], (hq + 2 * hkv) * d, dtype=dtype)
-    q, k, v = (y.unflatten(1, (-1, d)) for y in x.split((hq * d, hkv * d, hkv * d), 1))
+    x = _randn(rng, ends[-1], (hq + 2 * hkv) * d + 8, dtype=dtype)
+    q, k, v = (y.unflatten(1, (-1, d)) for y in x[:, :-8].split((hq * d, hkv * d, hkv * d), 1))
     out = ga.prompt_attention(q, k, v, _dev(ends))
     _check_prompt(out, q, k, v, ends, ends, dtype)
 
