@@ -196,7 +196,9 @@ int grinqh_gemm_or_gemv_noalloc(const void* x, int64_t M, int64_t K, int64_t ldx
  * attention over whole prompts.  head_dim is 64, 128 or 256; q, k and v rows are
  * [token][head][head_dim] with the given element distances of tokens and heads
  * (multiples of 8, at most 2^23; 16-byte aligned, channels adjacent), as slices
- * of a fused projection are; results are dense.
+ * of a fused projection are; results are dense.  As in all entry points the
+ * stream and the pointers belong to the device that is current in the calling
+ * thread.
  *
  * The cache is uint8 [pages][kv_heads][page_size / 16][record], page_size 16
  * times a power of two, 64-byte aligned.  A record (grinqh_kv4_record_bytes)

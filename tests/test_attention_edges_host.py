@@ -1,0 +1,74 @@
+"""CPU checks of the attention operators' host path at its edges: which device
+the library is called on, which inputs are copied or refused, what workspaces
+cover."""
+import pytest
+import torch
+
+from grinqh import _lib
+from grinqh import attention as ga
+
+SECOND = torch.device("cuda", 1)
+
+
+class OnSecond(torch.Tensor):
+    """A host tensor that says it is on the second GPU."""
+    is_cuda = True
+    device = SECOND
+
+
+def _second(*shape, dtype=torch.float16):
+    return torch.zeros(shape, dtype=dtype).as_subclass(OnSecond)
+
+
+class Devices:
+    """Stands in for the current device and for the library; notes the device of every C call."""
+
+    def __init__(self, monkeypatch, module):
+        self.current, self.calls = 0, []
+        here, empty = self, torch.empty
+
+        class Guard:
+            def __init__(self, device):
+                self.device = device
+
+            def __enter__(self):
+                self.before, here.current = here.current, self.device.index
+
+            def __exit__(self, *error):
+                here.current = self.before
+
+        class Library:
+            def __getattr__(self, name):
+                if name.endswith("bytes"):
+                    return lambda *args: 1024
+                return lambda *args: here.calls.append((name, here.current)) or 0
+
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: self.current, raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+        monkeypatch.setattr(torch.cuda, "device", Guard)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        for make in ("empty", "zeros"):
+            original = getattr(torch, make)
+            monkeypatch.setattr(torch, make, lambda *a, device=None, original=original, **k: original(*a, **k))
+        monkeypatch.setattr(torch, "empty_like", lambda x, **k: empty(x.shape, dtype=x.dtype))
+        monkeypatch.setattr(_lib, "load_library", lambda: Library())
+        if hasattr(module, "_stream"):
+            monkeypatch.setattr(module, "_stream", lambda device: 0)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_attention_runs_on_the_tensors_device(monkeypatch, current):
+    cache, q, k = _second(2, 2, 1, 2176, dtype=torch.uint8), _second(3, 8, 128), _second(3, 2, 128)
+    slots, lengths, table = (_second(*s, dtype=d) for s, d in (((3,), torch.int64), ((3,), torch.int32),
+                                                             ((3, 4), torch.int32)))
+    devices = Devices(monkeypatch, ga)
+    devices.current = current
+    ga._workspace_bytes.cache_clear()
+    ga.kv4_store(cache, k, k, slots)
+    ga.kv4_load(cache, slots)
+    ga.kv4_attention(q, cache, table, lengths)
+    ga.prompt_attention(q, k, k, lengths)
+    ga._workspace_bytes.cache_clear()
+    ga._WORKSPACES._bufs.clear()
+    assert devices.calls == [(f"grinqh_{n}", 1) for n in ("kv4_store", "kv4_load", "kv4_attention", "prompt_attention")]
+    assert devices.current == current

@@ -116,9 +116,10 @@ def kv4_store(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torc
         raise ValueError(f"GRINQH: k and v must be [tokens, {heads}, {d}] for this cache, got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
     slots = _index(slots, "slots", torch.int64, n, dev)
-    _lib.check(_lib.load_library().grinqh_kv4_store(
-        k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, slots.data_ptr(), n, cache.data_ptr(), pages,
-        heads, page, d, group, dt, _stream(dev.index)), "grinqh_kv4_store")
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().grinqh_kv4_store(
+            k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, slots.data_ptr(), n, cache.data_ptr(), pages,
+            heads, page, d, group, dt, _stream(dev.index)), "grinqh_kv4_store")
 
 
 def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
@@ -131,9 +132,10 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     slots = _index(slots, "slots", torch.int64, n, dev)
     k = torch.empty((n, heads, d), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    _lib.check(_lib.load_library().grinqh_kv4_load(
-        cache.data_ptr(), pages, heads, page, d, group, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt,
-        _stream(dev.index)), "grinqh_kv4_load")
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().grinqh_kv4_load(
+            cache.data_ptr(), pages, heads, page, d, group, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt,
+            _stream(dev.index)), "grinqh_kv4_load")
     return k, v
 
 
@@ -160,14 +162,15 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
     width = page_table.shape[1]
     out = torch.empty((seqs, heads, d), dtype=dtype, device=dev)
-    stream = _stream(dev.index)
-    nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
-    ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
-    _lib.check(_lib.load_library().grinqh_kv4_attention(
-        q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
-        page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
-        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
-        "grinqh_kv4_attention")
+    with _lib.on_device(dev):
+        stream = _stream(dev.index)
+        nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
+        ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
+        _lib.check(_lib.load_library().grinqh_kv4_attention(
+            q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
+            page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
+            "grinqh_kv4_attention")
     return out
 
 
@@ -205,8 +208,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
     else:
         key_ends = _index(key_ends, "key_ends", torch.int32, seqs + 1, dev)
     out = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
-    _lib.check(_lib.load_library().grinqh_prompt_attention(
-        q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, ends.data_ptr(),
-        key_ends.data_ptr(), seqs, tokens, keys, heads, kv_heads, d, _scale(scale, d), out.data_ptr(), dt,
-        _stream(dev.index)), "grinqh_prompt_attention")
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().grinqh_prompt_attention(
+            q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
+            ends.data_ptr(), key_ends.data_ptr(), seqs, tokens, keys, heads, kv_heads, d, _scale(scale, d),
+            out.data_ptr(), dt, _stream(dev.index)), "grinqh_prompt_attention")
     return out
