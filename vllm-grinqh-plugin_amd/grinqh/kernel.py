@@ -164,12 +164,13 @@ def run_product(x: torch.Tensor, weight_packed: torch.Tensor, weight_scale: torc
     mode_code = _MODES[mode]
     stream = torch._C._cuda_getCurrentRawStream(x.device.index)  # current_stream() without its wrapper object
     nbytes = _workspace_bytes(lib, M, K, N, max_bits, mode_code)
-    ws = _WORKSPACES.get(x.device, stream, nbytes)
-    _lib.check(lib.grinqh_gemm_or_gemv(
-        x2.data_ptr(), M, K, x2.stride(0), N, dt, wp.data_ptr(), scale.data_ptr(), bp, y.data_ptr(),
-        max_bits, group_size, _lib.thresholds_f32(thresholds), mode_code,
-        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
-        "grinqh_gemm_or_gemv")
+    with _lib.on_device(x.device):
+        ws = _WORKSPACES.get(x.device, stream, nbytes)
+        _lib.check(lib.grinqh_gemm_or_gemv(
+            x2.data_ptr(), M, K, x2.stride(0), N, dt, wp.data_ptr(), scale.data_ptr(), bp, y.data_ptr(),
+            max_bits, group_size, _lib.thresholds_f32(thresholds), mode_code,
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
+            "grinqh_gemm_or_gemv")
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 

@@ -45,10 +45,11 @@ def rmsnorm_sigma(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
         r_in = residual.reshape(-1, K).to(x.dtype).contiguous()
         r_out = torch.empty_like(r_in)
     lib = _lib.load_library()
-    _lib.check(lib.grinqh_rmsnorm_sigma(x2.data_ptr(), M, K, K, r_in.data_ptr() if r_in is not None else None,
-                                        r_out.data_ptr() if r_out is not None else None, w.data_ptr(), float(eps),
-                                        y.data_ptr(), sig.data_ptr(), _dtype_code(x.dtype), _stream(x.device)),
-               "grinqh_rmsnorm_sigma")
+    with _lib.on_device(x.device):
+        _lib.check(lib.grinqh_rmsnorm_sigma(x2.data_ptr(), M, K, K, r_in.data_ptr() if r_in is not None else None,
+                                            r_out.data_ptr() if r_out is not None else None, w.data_ptr(), float(eps),
+                                            y.data_ptr(), sig.data_ptr(), _dtype_code(x.dtype), _stream(x.device)),
+                   "grinqh_rmsnorm_sigma")
     return y.view(x.shape), sig, (r_out.view(x.shape) if r_out is not None else None)
 
 
@@ -66,9 +67,10 @@ def silu_mul_sigma(gate_up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     y = torch.empty((M, F), dtype=gate_up.dtype, device=gate_up.device)
     sig = torch.empty((_chunks(M), F), dtype=torch.float32, device=gate_up.device)
     lib = _lib.load_library()
-    _lib.check(lib.grinqh_silu_mul_sigma(g2.data_ptr(), M, F, F2, y.data_ptr(), sig.data_ptr(),
-                                         _dtype_code(gate_up.dtype), _stream(gate_up.device)),
-               "grinqh_silu_mul_sigma")
+    with _lib.on_device(gate_up.device):
+        _lib.check(lib.grinqh_silu_mul_sigma(g2.data_ptr(), M, F, F2, y.data_ptr(), sig.data_ptr(),
+                                             _dtype_code(gate_up.dtype), _stream(gate_up.device)),
+                   "grinqh_silu_mul_sigma")
     return y.view(*gate_up.shape[:-1], F), sig
 
 
@@ -95,11 +97,12 @@ def gemv_batch_union_sigma(x: torch.Tensor, weight_packed: torch.Tensor, weight_
     lib = _lib.load_library()
     stream = _stream(x.device)
     nbytes = lib.grinqh_workspace_bytes(M, K, N, max_bits, _lib.MODE_UNION)
-    ws = _WORKSPACES.get(x.device, stream, nbytes)
-    _lib.check(lib.grinqh_gemv_batch_union_sigma(
-        x2.data_ptr(), M, K, K, N, _dtype_code(x.dtype), wp.data_ptr(), scale.data_ptr(),
-        b.data_ptr() if b is not None else None,
-        y.data_ptr(), max_bits, group_size, _lib.thresholds_f32(thresholds), sc.data_ptr(),
-        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
-        "grinqh_gemv_batch_union_sigma")
+    with _lib.on_device(x.device):
+        ws = _WORKSPACES.get(x.device, stream, nbytes)
+        _lib.check(lib.grinqh_gemv_batch_union_sigma(
+            x2.data_ptr(), M, K, K, N, _dtype_code(x.dtype), wp.data_ptr(), scale.data_ptr(),
+            b.data_ptr() if b is not None else None,
+            y.data_ptr(), max_bits, group_size, _lib.thresholds_f32(thresholds), sc.data_ptr(),
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
+            "grinqh_gemv_batch_union_sigma")
     return y.view(*x.shape[:-1], N)

@@ -59,8 +59,9 @@ def pack_planes(A: torch.Tensor, max_bits: int = 8) -> torch.Tensor:
     K = A.shape[0]
     N = A.shape[1] * A.element_size()
     out = torch.empty((K, (max_bits // 2) * (N // 16)), device=A.device, dtype=torch.uint32)
-    _lib.check(_lib.load_library().grinqh_pack_planes(A.data_ptr(), out.data_ptr(), K, N, max_bits,
-                                                      _stream(A.device)), "grinqh_pack_planes")
+    with _lib.on_device(A.device):
+        _lib.check(_lib.load_library().grinqh_pack_planes(A.data_ptr(), out.data_ptr(), K, N, max_bits,
+                                                          _stream(A.device)), "grinqh_pack_planes")
     return out
 
 
@@ -74,8 +75,9 @@ def prepare_weight(w_int8: torch.Tensor, max_bits: int = 8) -> torch.Tensor:
     if N % 16 != 0:
         raise AssertionError("N must be divisible by 16 for this layout.")
     out = torch.empty((K, (max_bits // 2) * (N // 16)), device=w.device, dtype=torch.uint32)
-    _lib.check(_lib.load_library().grinqh_prepare_weight(w.data_ptr(), out.data_ptr(), K, N, max_bits,
-                                                         _stream(w.device)), "grinqh_prepare_weight")
+    with _lib.on_device(w.device):
+        _lib.check(_lib.load_library().grinqh_prepare_weight(w.data_ptr(), out.data_ptr(), K, N, max_bits,
+                                                             _stream(w.device)), "grinqh_prepare_weight")
     return out
 
 
@@ -94,9 +96,10 @@ def unpack_planes(B: torch.Tensor, row: Union[int, torch.Tensor], bit_level: Bit
         raise IndexError(f"GRINQH unpack: row index out of range [0, {B.shape[0]})")
     out = torch.empty((rows.numel(), original_n), device=B.device, dtype=torch.uint32)
     Bc = B.contiguous()
-    _lib.check(_lib.load_library().grinqh_unpack_planes(Bc.data_ptr(), rows.data_ptr(), rows.numel(),
-                                                        out.data_ptr(), Bc.shape[0], N, int(bit_level.value),
-                                                        _stream(B.device)), "grinqh_unpack_planes")
+    with _lib.on_device(B.device):
+        _lib.check(_lib.load_library().grinqh_unpack_planes(Bc.data_ptr(), rows.data_ptr(), rows.numel(),
+                                                            out.data_ptr(), Bc.shape[0], N, int(bit_level.value),
+                                                            _stream(B.device)), "grinqh_unpack_planes")
     return out
 
 
@@ -116,9 +119,10 @@ def dequantize(weight_packed: torch.Tensor, weight_scale: torch.Tensor | None, m
         out = torch.empty((K, N), device=weight_packed.device, dtype=dtype)
         sp = weight_scale.contiguous().data_ptr()
         dt = _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F16
-    _lib.check(_lib.load_library().grinqh_dequantize(weight_packed.contiguous().data_ptr(), sp, out.data_ptr(), K, N,
-                                                     max_bits, group_size, dt, _stream(weight_packed.device)),
-               "grinqh_dequantize")
+    with _lib.on_device(weight_packed.device):
+        _lib.check(_lib.load_library().grinqh_dequantize(weight_packed.contiguous().data_ptr(), sp, out.data_ptr(), K,
+                                                         N, max_bits, group_size, dt, _stream(weight_packed.device)),
+                   "grinqh_dequantize")
     return out
 
 
@@ -134,7 +138,8 @@ def grade(x: torch.Tensor, thresholds, max_bits: int):
     dt = _lib.DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.DTYPE_F16
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("GRINQH activations must be float16 or bfloat16")
-    _lib.check(_lib.load_library().grinqh_grade(x2.data_ptr(), M, K, K, dt, max_bits,
-                                                _lib.thresholds_f32(thresholds), bits.data_ptr(),
-                                                beta.data_ptr(), _stream(x.device)), "grinqh_grade")
+    with _lib.on_device(x.device):
+        _lib.check(_lib.load_library().grinqh_grade(x2.data_ptr(), M, K, K, dt, max_bits,
+                                                    _lib.thresholds_f32(thresholds), bits.data_ptr(),
+                                                    beta.data_ptr(), _stream(x.device)), "grinqh_grade")
     return bits, beta
