@@ -246,7 +246,8 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
  * device, ascending; the same array for plain prompts).  The last rows are
  * aligned with the last keys: row i of R sees keys 0 .. i + (K - R) of K, none
  * when that is negative (zeros).  Rows behind the last sequence give zeros.
- * Offsets are limited to the tensors.  k_token and v_token are at least
+ * Keys and values that a row does not see have no effect on it, whatever they
+ * hold.  Offsets are limited to the tensors.  k_token and v_token are at least
  * head_dim; scale > 0. */
 int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                             int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* q_ends,

@@ -1,0 +1,51 @@
+"""GPU tests of the attention operators at the edges of their inputs: values
+and rows that must not count, layouts of memory, extreme magnitudes, runs
+joined over many blocks.  The oracles and bounds are those of
+test_attention_gpu.py; where two calls must agree, they agree bit for bit."""
+import numpy as np
+import pytest
+import torch
+
+from test_attention_gpu import DT, LIMIT, _check_decode, _check_prompt, _dev, _ends, _paged, _params, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a HIP device")
+
+
+# ---------------------------------------------------------------- values that a row must not see
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,keys", [(300, 300), (70, 333), (290, 200), (1, 65), (20, 20)])
+def test_prompt_later_values_do_not_count(dtype, d, rows, keys):
+    """NaN and infinities in values: in the channels of the rows that see them, as the sum gives them, and nowhere
+    else, whatever tile the rows share with them"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(rows + keys + d)
+    hq, hkv = 4, 2
+    ends, key_ends = [0, 17, 17 + rows], [0, 30, 30 + keys]
+    q = _randn(rng, ends[-1], hq, d, dtype=dtype)
+    k, v = (_randn(rng, key_ends[-1], hkv, d, dtype=dtype) for _ in (0, 1))
+    nan, inf = float("nan"), float("inf")
+    spots = [(0, 0, 3, nan), (1, 1, 4, inf), (5, 0, 9, -inf), (40, 1, 63, nan), (63, 0, 20, inf), (64, 0, 21, -inf),
+             (64, 1, 21, inf), (100, 1, 21, -inf), (127, 0, 8, nan), (128, 1, 5, inf), (150, 0, 8, inf),
+             (199, 0, 33, nan), (keys - 1, 0, 2, nan), (keys - 1, 1, 1, inf), (keys - 2, 1, 62, -inf)]
+    spots = [s for s in spots if 0 <= s[0] < keys]
+    bad, none = v.clone(), v.clone()
+    effect = torch.zeros_like(q, dtype=torch.float32)
+    row = torch.arange(rows, device="cuda")
+    for key, head, channel, value in spots:
+        bad[30 + key, head, channel] = value
+        none[30 + key, head, channel] = 0.0
+        seen = torch.where(row + keys - rows >= key, value, 0.0).view(-1, 1)
+        effect[17:, 2 * head:2 * head + 2, channel] += seen
+    out = ga.prompt_attention(q, k, bad, _dev(ends), _dev(key_ends))
+    want = ga.prompt_attention(q, k, none, _dev(ends), _dev(key_ends)) + effect.to(q.dtype)
+    assert bool(want.isfinite().any())
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(0.0, inf, -inf), want.nan_to_num(0.0, inf, -inf))

@@ -149,7 +149,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
   // separate arrays, used by name: the compiler's wait for a tile that was loaded
   // straight into LDS is then not one for the tiles still on their way
   __shared__ __align__(1024) uint8_t s_k0[KEY_TILE], s_k1[KEY_TILE], s_v0[VALUE_TILE], s_v1[VALUE_TILE];
-  const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+  __shared__ __align__(16) int s_first[3][D];  // first key whose value is NaN, +inf, -inf, by channel
+  __shared__ int s_redo[kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // heads of one key/value head run on one XCD (its L2 then holds their keys and values)
@@ -164,227 +165,298 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     head = L % p.heads;
     index = L / p.heads;
   }
-  Sequence sq;
-  int64_t block;
-  if (find_block(p, index, lane, sq, block) < 0) return;
-  sq = {uniform(sq.row0), uniform(sq.key0), uniform(sq.rows), uniform(sq.keys)};
-  block = uniform(block);
-  const int kvh = head / (p.heads / p.kv_heads);
-  const int row0 = (int)block * kBlockRows + wave * 32;  // of this wave, in the sequence
-  const int rows = (int)sq.rows, shift = (int)(sq.keys - sq.rows), keys = (int)sq.keys;
-  // keys that the block's last row sees
-  const int block_keys = min(keys, min((int)(block + 1) * kBlockRows, rows) + shift);
-  const int tiles = block_keys > 0 ? (block_keys + kKeys - 1) / kKeys : 0;
-  const int wave_keys = row0 < rows ? min(keys, min(row0 + 32, rows) + shift) : 0;
+  // The block's rows; true if some result is NaN or infinite.  Two copies of the
+  // code, so that the second pass costs the first no registers.
+  auto attend = [&](auto second, int lane) __attribute__((always_inline)) -> bool {
+    constexpr bool APART = decltype(second)::value;
+    const int n = lane & 31, half = lane >> 5;
+    Sequence sq;
+    int64_t block;
+    if (find_block(p, index, lane, sq, block) < 0) return false;
+    sq = {uniform(sq.row0), uniform(sq.key0), uniform(sq.rows), uniform(sq.keys)};
+    block = uniform(block);
+    const int kvh = head / (p.heads / p.kv_heads);
+    const int row0 = (int)block * kBlockRows + wave * 32;  // of this wave, in the sequence
+    const int rows = (int)sq.rows, shift = (int)(sq.keys - sq.rows), keys = (int)sq.keys;
+    // keys that the block's last row sees
+    const int block_keys = min(keys, min((int)(block + 1) * kBlockRows, rows) + shift);
+    const int tiles = block_keys > 0 ? (block_keys + kKeys - 1) / kKeys : 0;
+    const int wave_keys = row0 < rows ? min(keys, min(row0 + 32, rows) + shift) : 0;
 
-  // queries: row n, channels 16 s + 8 half + e
-  u32x4_t qf[STEPS];
-  {
-    const uint16_t* q = p.q.p + (sq.row0 + min(row0 + n, rows - 1)) * p.q.token + (int64_t)head * p.q.head + 8 * half;
+    // queries: row n, channels 16 s + 8 half + e
+    u32x4_t qf[STEPS];
+    {
+      const uint16_t* q = p.q.p + (sq.row0 + min(row0 + n, rows - 1)) * p.q.token + (int64_t)head * p.q.head + 8 * half;
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s);
-  }
-
-  // LDS position of 16-byte chunk c of key r.  Loads straight into LDS put 1 KiB
-  // (PER keys) in a row, so what is read together is spread over the banks by
-  // flipping bits of c, and for the keys by a gap after every KiB as well: the
-  // keys' reads want 16 adjacent keys' chunks in 256 different bytes, the values'
-  // transposed reads 4 adjacent keys' 64 bytes.  Few bits are flipped, so that
-  // most of an address is an immediate offset.
-  auto key_swz = [](int r) { return D == 64 ? (r >> 1) & 3 : D == 128 ? r & 3 : r & 1; };
-  auto value_swz = [](int r) { return (D == 64 ? (r >> 1) & 1 : r & 3) << 2; };
-  auto key_at = [](int r) { return r / PER * KEY_GROUP + r % PER * (2 * D); };
-  const uint16_t* kbase = p.k.p + sq.key0 * p.k.token + (int64_t)kvh * p.k.head;
-  const uint16_t* vbase = p.v.p + sq.key0 * p.v.token + (int64_t)kvh * p.v.head;
-  // A wave loads PER keys at a time, 1 KiB; keys past the sequence's end come as
-  // zeros (behind the buffer's end, as rows are at least D apart).
-  const int load_row = wave * PER + lane / CHUNKS;
-  static_assert(kWaves * PER % 8 == 0, "the flipped bits are the same for all loads of a lane");
-  const int key_off = load_row * (int)p.k.token * 2 + (((lane % CHUNKS) ^ key_swz(load_row)) << 4);
-  const int value_off = load_row * (int)p.v.token * 2 + (((lane % CHUNKS) ^ value_swz(load_row)) << 4);
-  auto load_tile = [&](const uint16_t* base, int64_t stride, int off, int tile, uint8_t* to, int group) {
-#pragma unroll
-    for (int i = 0; i < kKeys / PER / kWaves; ++i) {
-      const int r0 = tile * kKeys + i * kWaves * PER, live = min(kKeys, keys - r0);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint16_t*>(base + (int64_t)r0 * stride), (short)0,
-          live > 0 ? (int)(((live - 1) * stride + D) * 2) : 0, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(to + (i * kWaves + wave) * group), 16, off, 0, 0, 0);
+      for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s);
     }
-  };
 
-  f32x16_t O[MT];
-  float M = kLow, sum = 0.f;
+    // LDS position of 16-byte chunk c of key r.  Loads straight into LDS put 1 KiB
+    // (PER keys) in a row, so what is read together is spread over the banks by
+    // flipping bits of c, and for the keys by a gap after every KiB as well: the
+    // keys' reads want 16 adjacent keys' chunks in 256 different bytes, the values'
+    // transposed reads 4 adjacent keys' 64 bytes.  Few bits are flipped, so that
+    // most of an address is an immediate offset.
+    auto key_swz = [](int r) { return D == 64 ? (r >> 1) & 3 : D == 128 ? r & 3 : r & 1; };
+    auto value_swz = [](int r) { return (D == 64 ? (r >> 1) & 1 : r & 3) << 2; };
+    auto key_at = [](int r) { return r / PER * KEY_GROUP + r % PER * (2 * D); };
+    const uint16_t* kbase = p.k.p + sq.key0 * p.k.token + (int64_t)kvh * p.k.head;
+    const uint16_t* vbase = p.v.p + sq.key0 * p.v.token + (int64_t)kvh * p.v.head;
+    // A wave loads PER keys at a time, 1 KiB; keys past the sequence's end come as
+    // zeros (behind the buffer's end, as rows are at least D apart).
+    const int load_row = wave * PER + lane / CHUNKS;
+    static_assert(kWaves * PER % 8 == 0, "the flipped bits are the same for all loads of a lane");
+    const int key_off = load_row * (int)p.k.token * 2 + (((lane % CHUNKS) ^ key_swz(load_row)) << 4);
+    const int value_off = load_row * (int)p.v.token * 2 + (((lane % CHUNKS) ^ value_swz(load_row)) << 4);
+    auto load_tile = [&](const uint16_t* base, int64_t stride, int off, int tile, uint8_t* to, int group) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m) O[m] = (f32x16_t)(0.f);
-  const float c2 = p.scale * 1.44269504088896f;
-  const int my_tiles = wave_keys > 0 ? (wave_keys + kKeys - 1) / kKeys : 0;
-
-  // LDS reads.  Keys: row n of key block b, channels 16 s + 8 half + e.  Values,
-  // transposed: channel 32 m + n, keys 16 t + 4 half + 0..3 and + 8.
-  // The flipped bits make two bases (four for the values), the rest are offsets.
-  int key_base[2], value_base[4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) key_base[i] = key_at(n) + (((2 * i + half) ^ key_swz(n)) << 4);
-  const int vrow = 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    value_base[i] = vrow * D * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ value_swz(vrow)) << 4) +
-                    8 * (lane & 1);
-  auto read_key = [&](const uint8_t* kt, int b, int s) {
-    return *reinterpret_cast<const u32x4_t*>(kt + key_base[s & 1] + key_at(32 * b) + 64 * (s >> 1));
-  };
-  auto read_value = [&](const uint8_t* vt, int t, int m) {
-    u32x4_t a;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s16x4_t)(vt + value_base[m & 3] + (16 * t + 8 * u) * D * 2 + 256 * (m >> 2)));
-      const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
-      a[2 * u] = y[0];
-      a[2 * u + 1] = y[1];
-    }
-    return a;
-  };
-  u32x4_t P[4];
-  // weights of two keys: pair q of key block b
-  auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], c2, -M));
-    const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], c2, -M));
-    sum += p0 + p1;
-    P[2 * b + (q >> 2)][q & 3] = pack2<DT>(p0, p1);
-  };
-  // Makes S of a tile ready for its weights: the mask where the tile reaches
-  // past a row's last key, and the reference raised where a weight would pass
-  // 2^8 (rarely after the first tiles: the accumulators are not rescaled for less).
-  auto settle = [&](f32x16_t (&S)[2], float& top, int tile) {
-    if (tile * kKeys + kKeys - 1 > row0 + shift) {
-      // last key of this tile that the row sees, less the half's 4 (compared with constants)
-      const int seen = row0 + n + shift - tile * kKeys - 4 * half;
-      top = -__builtin_inff();
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (32 * b + (e & 3) + 8 * (e >> 2) > seen) S[b][e] = -__builtin_inff();
-          top = fmaxf(top, S[b][e]);
-        }
-    }
-    if (__any(fmaf(top, c2, -M) > 8.f)) {
-      float m = fmaxf(M, top * c2);
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float f = __builtin_amdgcn_exp2f(M - m);
-      M = m;
-      sum *= f;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) O[t] *= f;
-    }
-  };
-
-  // One tile: its weights and its part of O, and the products of the next tile,
-  // slot by slot: every slot gives the matrix unit one product and the vector unit
-  // a share of the exponentials (those of keys 0..31 under the next tile's
-  // products, those of keys 32..63 under the first values'), with LDS reads AHEAD
-  // slots before their use (1: 571 us, 2: 539, 3: 533 at one sequence of 8192 rows,
-  // 32 heads of 128).
-  constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = 3;
-  auto step = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], const uint8_t* kt, const uint8_t* vt, float& top) {
-    u32x4_t f[AHEAD + 1];
-    auto read = [&](int at) {  // the A operand of slot `at`
-      f[at % (AHEAD + 1)] = at < KSLOTS ? read_key(kt, at / STEPS, at % STEPS)
-                                        : read_value(vt, (at - KSLOTS) / MT, (at - KSLOTS) % MT);
+      for (int i = 0; i < kKeys / PER / kWaves; ++i) {
+        const int r0 = tile * kKeys + i * kWaves * PER, live = min(kKeys, keys - r0);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(base + (int64_t)r0 * stride), (short)0,
+            live > 0 ? (int)(((live - 1) * stride + D) * 2) : 0, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(to + (i * kWaves + wave) * group), 16, off, 0, 0, 0);
+      }
     };
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) read(k);
-    int done = 0;
-#pragma unroll
-    for (int k = 0; k < KSLOTS; ++k) {
-      const int b = k / STEPS, s = k % STEPS;
-      read(k + AHEAD);
-      N[b] = mfma32x32x16<DT>(f[k % (AHEAD + 1)], qf[s], s == 0 ? (f32x16_t)(0.f) : N[b]);
-#pragma unroll
-      for (; done < (k + 1) * 8 / KSLOTS; ++done) weigh(S, 0, done);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    done = 0;
-    int seen = 0;
-    top = -__builtin_inff();
-#pragma unroll
-    for (int k = 0; k < VSLOTS; ++k) {
-      const int t = k / MT, m = k % MT;
-      if (k + AHEAD < VSLOTS) read(KSLOTS + k + AHEAD);
-      O[m] = mfma32x32x16<DT>(f[(KSLOTS + k) % (AHEAD + 1)], P[t], O[m]);
-      if (k < VSLOTS / 2) {
-#pragma unroll
-        for (; done < (k + 1) * 8 / (VSLOTS / 2); ++done) weigh(S, 1, done);
-      } else {
-#pragma unroll
-        for (; seen < (k + 1 - VSLOTS / 2) * 16 / (VSLOTS / 2); ++seen)
-          top = fmaxf(fmaxf(top, N[seen >> 3][2 * (seen & 7)]), N[seen >> 3][2 * (seen & 7) + 1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
 
-  // Keys run one tile ahead of the values: while tile j is weighed, S of tile
-  // j + 1 is computed and the keys of j + 2 and the values of j + 1 are loaded.
-  // After the wave's last tile S is computed from whatever LDS holds, and not used:
-  // a second form of the step would cost the registers of a second O.
-  f32x16_t Sa[2], Sb[2];
-  float top;
-  if (tiles > 0) {
-    load_tile(kbase, p.k.token, key_off, 0, s_k0, KEY_GROUP);
-    load_tile(vbase, p.v.token, value_off, 0, s_v0, 1024);
-    if (tiles > 1) load_tile(kbase, p.k.token, key_off, 1, s_k1, KEY_GROUP);
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's shares are in LDS
-    __syncthreads();
-    if (my_tiles > 0) {
+    f32x16_t O[MT];
+    float M = kLow, sum = 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) O[m] = (f32x16_t)(0.f);
+    const float c2 = p.scale * 1.44269504088896f;
+    const int my_tiles = wave_keys > 0 ? (wave_keys + kKeys - 1) / kKeys : 0;
+
+    // LDS reads.  Keys: row n of key block b, channels 16 s + 8 half + e.  Values,
+    // transposed: channel 32 m + n, keys 16 t + 4 half + 0..3 and + 8.
+    // The flipped bits make two bases (four for the values), the rest are offsets.
+    int key_base[2], value_base[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) key_base[i] = key_at(n) + (((2 * i + half) ^ key_swz(n)) << 4);
+    const int vrow = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      value_base[i] = vrow * D * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ value_swz(vrow)) << 4) +
+                      8 * (lane & 1);
+    auto read_key = [&](const uint8_t* kt, int b, int s) {
+      return *reinterpret_cast<const u32x4_t*>(kt + key_base[s & 1] + key_at(32 * b) + 64 * (s >> 1));
+    };
+    auto read_value = [&](const uint8_t* vt, int t, int m) {
+      u32x4_t a;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4_t)(vt + value_base[m & 3] + (16 * t + 8 * u) * D * 2 + 256 * (m >> 2)));
+        const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
+        a[2 * u] = y[0];
+        a[2 * u + 1] = y[1];
+      }
+      return a;
+    };
+    u32x4_t P[4];
+    // weights of two keys: pair q of key block b
+    auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], c2, -M));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], c2, -M));
+      sum += p0 + p1;
+      P[2 * b + (q >> 2)][q & 3] = pack2<DT>(p0, p1);
+    };
+    // Makes S of a tile ready for its weights: the mask where the tile reaches
+    // past a row's last key, and the reference raised where a weight would pass
+    // 2^8 (rarely after the first tiles: the accumulators are not rescaled for less).
+    auto settle = [&](f32x16_t (&S)[2], float& top, int tile) {
+      if (tile * kKeys + kKeys - 1 > row0 + shift) {
+        // last key of this tile that the row sees, less the half's 4 (compared with constants)
+        const int seen = row0 + n + shift - tile * kKeys - 4 * half;
+        top = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (32 * b + (e & 3) + 8 * (e >> 2) > seen) S[b][e] = -__builtin_inff();
+            top = fmaxf(top, S[b][e]);
+          }
+      }
+      if (__any(fmaf(top, c2, -M) > 8.f)) {
+        float m = fmaxf(M, top * c2);
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float f = __builtin_amdgcn_exp2f(M - m);
+        M = m;
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) O[t] *= f;
+      }
+    };
+
+    // One tile: its weights and its part of O, and the products of the next tile,
+    // slot by slot: every slot gives the matrix unit one product and the vector unit
+    // a share of the exponentials (those of keys 0..31 under the next tile's
+    // products, those of keys 32..63 under the first values'), with LDS reads AHEAD
+    // slots before their use (1: 571 us, 2: 539, 3: 533 at one sequence of 8192 rows,
+    // 32 heads of 128).
+    constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = 3;
+    auto step = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], const uint8_t* kt, const uint8_t* vt, float& top) {
+      u32x4_t f[AHEAD + 1];
+      auto read = [&](int at) {  // the A operand of slot `at`
+        f[at % (AHEAD + 1)] = at < KSLOTS ? read_key(kt, at / STEPS, at % STEPS)
+                                          : read_value(vt, (at - KSLOTS) / MT, (at - KSLOTS) % MT);
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) read(k);
+      int done = 0;
+#pragma unroll
+      for (int k = 0; k < KSLOTS; ++k) {
+        const int b = k / STEPS, s = k % STEPS;
+        read(k + AHEAD);
+        N[b] = mfma32x32x16<DT>(f[k % (AHEAD + 1)], qf[s], s == 0 ? (f32x16_t)(0.f) : N[b]);
+#pragma unroll
+        for (; done < (k + 1) * 8 / KSLOTS; ++done) weigh(S, 0, done);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      done = 0;
+      int seen = 0;
       top = -__builtin_inff();
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        Sa[b] = (f32x16_t)(0.f);
+      for (int k = 0; k < VSLOTS; ++k) {
+        const int t = k / MT, m = k % MT;
+        if (k + AHEAD < VSLOTS) read(KSLOTS + k + AHEAD);
+        O[m] = mfma32x32x16<DT>(f[(KSLOTS + k) % (AHEAD + 1)], P[t], O[m]);
+        if (k < VSLOTS / 2) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) Sa[b] = mfma32x32x16<DT>(read_key(s_k0, b, s), qf[s], Sa[b]);
+          for (; done < (k + 1) * 8 / (VSLOTS / 2); ++done) weigh(S, 1, done);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, Sa[b][e]);
+          for (; seen < (k + 1 - VSLOTS / 2) * 16 / (VSLOTS / 2); ++seen)
+            top = fmaxf(fmaxf(top, N[seen >> 3][2 * (seen & 7)]), N[seen >> 3][2 * (seen & 7) + 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      settle(Sa, top, 0);
-    }
-  }
-  // k, v: where tile j is; v_next: the values' other slot
-  auto turn = [&](int j, uint8_t* k, uint8_t* v_next) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    if (j + 2 < tiles) load_tile(kbase, p.k.token, key_off, j + 2, k, KEY_GROUP);
-    if (j + 1 < tiles) load_tile(vbase, p.v.token, value_off, j + 1, v_next, 1024);
-  };
-  int j = 0;
-  for (; j + 1 < my_tiles; j += 2) {
-    turn(j, s_k0, s_v1);
-    step(Sa, Sb, s_k1, s_v0, top);
-    settle(Sb, top, j + 1);
-    turn(j + 1, s_k1, s_v0);
-    step(Sb, Sa, s_k0, s_v1, top);
-    if (j + 2 < my_tiles) settle(Sa, top, j + 2);
-  }
-  if (j < my_tiles) {
-    turn(j, s_k0, s_v1);
-    step(Sa, Sb, s_k1, s_v0, top);
-    ++j;
-  }
-  for (; j < tiles; ++j) turn(j, (j & 1) ? s_k1 : s_k0, (j & 1) ? s_v0 : s_v1);  // the other waves' tiles
+    };
 
-  const float l = sum + __shfl_xor(sum, 32, 64);
-  const int row = row0 + n;
-  if (row >= rows) return;
-  const float inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees no key gives zeros
-  uint16_t* o = p.out + ((sq.row0 + row) * p.heads + head) * D + 4 * half;
+    // A value that is NaN or infinite must not reach the rows that do not see its
+    // key, but their weight of zero times it is NaN.  Such results send the block
+    // through its keys a second time (so do rows that see one): with `apart`, tiles
+    // that not all rows see whole are stripped of these values, which keep their
+    // place in s_first: key j is seen by the rows from j - shift on, so that the
+    // first key of each kind and channel decides.
+    auto strip = [&](uint8_t* vt, int tile) {
+      constexpr uint32_t kInf = DT::id == F16::id ? 0x7C00u : 0x7F80u;
+      int at = 64 * wave + lane;
+      asm volatile("" : "+v"(at));  // addresses are computed here, not kept through the products
+#pragma unroll 1
+      for (; at < VALUE_TILE / 16; at += 64 * kWaves) {
+        const int r = at / CHUNKS, c = (at % CHUNKS) ^ value_swz(r);
+        u32x4_t* place = reinterpret_cast<u32x4_t*>(vt) + at;
+        u32x4_t w = *place;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t x = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+          if ((x & kInf) == kInf) {
+            atomicMin(&s_first[(x & 0x7FFFu) > kInf ? 0 : 1 + (int)(x >> 15)][8 * c + e], tile * kKeys + r);
+            w[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          }
+        }
+        *place = w;
+      }
+    };
+
+    // Keys run one tile ahead of the values: while tile j is weighed, S of tile
+    // j + 1 is computed and the keys of j + 2 and the values of j + 1 are loaded.
+    // After the wave's last tile S is computed from whatever LDS holds, and not used:
+    // a second form of the step would cost the registers of a second O.
+    f32x16_t Sa[2], Sb[2];
+    float top;
+    if constexpr (APART)
+#pragma unroll 1
+      for (int i = 64 * wave + lane; i < 3 * D; i += 64 * kWaves) s_first[0][i] = INT32_MAX;
+    if (tiles > 0) {
+      load_tile(kbase, p.k.token, key_off, 0, s_k0, KEY_GROUP);
+      load_tile(vbase, p.v.token, value_off, 0, s_v0, 1024);
+      if (tiles > 1) load_tile(kbase, p.k.token, key_off, 1, s_k1, KEY_GROUP);
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's shares are in LDS
+      __syncthreads();
+      if (my_tiles > 0) {
+        top = -__builtin_inff();
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) = u32x2_t{
-          pack2<DT>(O[m][e] * inv, O[m][e + 1] * inv), pack2<DT>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
+        for (int b = 0; b < 2; ++b) {
+          Sa[b] = (f32x16_t)(0.f);
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) Sa[b] = mfma32x32x16<DT>(read_key(s_k0, b, s), qf[s], Sa[b]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, Sa[b][e]);
+        }
+        settle(Sa, top, 0);
+      }
+    }
+    // k, v: where tile j is; v_next: the values' other slot
+    auto turn = [&](int j, uint8_t* k, uint8_t* v, uint8_t* v_next) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      __syncthreads();
+      if (APART && j * kKeys + kKeys - 1 > (int)block * kBlockRows + shift) {
+        strip(v, j);
+        __syncthreads();
+      }
+      if (j + 2 < tiles) load_tile(kbase, p.k.token, key_off, j + 2, k, KEY_GROUP);
+      if (j + 1 < tiles) load_tile(vbase, p.v.token, value_off, j + 1, v_next, 1024);
+    };
+    int j = 0;
+    for (; j + 1 < my_tiles; j += 2) {
+      turn(j, s_k0, s_v0, s_v1);
+      step(Sa, Sb, s_k1, s_v0, top);
+      settle(Sb, top, j + 1);
+      turn(j + 1, s_k1, s_v1, s_v0);
+      step(Sb, Sa, s_k0, s_v1, top);
+      if (j + 2 < my_tiles) settle(Sa, top, j + 2);
+    }
+    if (j < my_tiles) {
+      turn(j, s_k0, s_v0, s_v1);
+      step(Sa, Sb, s_k1, s_v0, top);
+      ++j;
+    }
+    for (; j < tiles; ++j)  // the other waves' tiles
+      turn(j, (j & 1) ? s_k1 : s_k0, (j & 1) ? s_v1 : s_v0, (j & 1) ? s_v0 : s_v1);
+
+    const float l = sum + __shfl_xor(sum, 32, 64);
+    const int row = row0 + n;
+    const float inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees no key gives zeros
+    float odd = 0.f;  // NaN if an accumulator is NaN or infinite
+    uint16_t* o = p.out + ((sq.row0 + row) * p.heads + head) * D + 4 * half;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        u32x2_t w =
+            u32x2_t{pack2<DT>(O[m][e] * inv, O[m][e + 1] * inv), pack2<DT>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          odd = fmaf(O[m][e + i], 0.f, odd);
+          if constexpr (APART) {
+            const int channel = 32 * m + 2 * e + 4 * half + i, seen = row + shift;
+            const bool nan = s_first[0][channel] <= seen, up = s_first[1][channel] <= seen,
+                       down = s_first[2][channel] <= seen;
+            float x = to_f32<DT>((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+            if (up) x += __builtin_inff();
+            if (down) x -= __builtin_inff();
+            if (nan) x = __builtin_nanf("");
+            if (nan || up || down)
+              w[i >> 1] = i & 1 ? (w[i >> 1] & 0xFFFFu) | ((uint32_t)from_f32<DT>(x) << 16)
+                                : (w[i >> 1] & 0xFFFF0000u) | from_f32<DT>(x);
+          }
+        }
+        if (row < rows) *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) = w;
+      }
+    if (APART || tiles == 0) return false;
+    const int mine = __any(odd != odd);
+    if (lane == 0) s_redo[wave] = mine;
+    __syncthreads();
+    int redo = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) redo |= s_redo[w];
+    return redo != 0;
+  };
+  if (!attend(std::false_type{}, threadIdx.x & 63)) return;
+  int none = 0;
+  asm volatile("" : "+s"(index), "+s"(head), "+s"(none));  // nothing is kept from the first pass
+  attend(std::true_type{}, __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)));
 }
 
 }  // namespace
