@@ -245,7 +245,8 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
  * of q attend to keys k_ends[s] .. k_ends[s + 1] - 1 (int32 [seqs + 1] each,
  * device, ascending; the same array for plain prompts).  The last rows are
  * aligned with the last keys: row i of R sees keys 0 .. i + (K - R) of K, none
- * when that is negative (zeros).  Rows behind the last sequence give zeros.
+ * when that is negative (zeros).  Rows in front of the first sequence (q_ends[0]
+ * > 0) and behind the last give zeros.
  * Keys and values that a row does not see have no effect on it, whatever they
  * hold.  Offsets are limited to the tensors.  k_token and v_token are at least
  * head_dim; scale > 0. */

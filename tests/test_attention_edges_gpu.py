@@ -49,3 +49,23 @@ def test_prompt_later_values_do_not_count(dtype, d, rows, keys):
     assert bool(want.isfinite().any())
     assert torch.equal(out.isnan(), want.isnan())
     assert torch.equal(out.nan_to_num(0.0, inf, -inf), want.nan_to_num(0.0, inf, -inf))
+
+
+# ---------------------------------------------------------------- rows of no sequence
+
+@pytest.mark.parametrize("ends", [[9, 40, 70], [300, 300, 333], [77], [200, 201], [1, 80, 80]])
+@pytest.mark.parametrize("heads", [4, 8])
+def test_prompt_rows_before_the_first_sequence(ends, heads):
+    """rows in front of the first sequence give zeros, as those behind the last do"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(ends[0])
+    tokens = ends[-1] + 50
+    q, k, v = (_randn(rng, tokens, n, 64) for n in (heads, 2, 2))
+    stale = torch.full((tokens, heads, 64), float("nan"), dtype=q.dtype, device="cuda")
+    del stale  # the result is likely to lie where this was
+    out = ga.prompt_attention(q, k, v, _dev(ends))
+    _check_prompt(out, q, k, v, ends, ends, "f16")
+    key_ends = [e - ends[0] for e in ends]
+    stale = torch.full((tokens, heads, 64), float("nan"), dtype=q.dtype, device="cuda")
+    del stale, out
+    _check_prompt(ga.prompt_attention(q, k, v, _dev(ends), _dev(key_ends)), q, k, v, ends, key_ends, "f16")

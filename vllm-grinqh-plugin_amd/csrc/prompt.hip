@@ -165,6 +165,17 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     head = L % p.heads;
     index = L / p.heads;
   }
+  // A head's first block: zeros for the rows in front of the first sequence, which
+  // are few.  The others need not wait for ends[0].
+  if (index == 0) {
+    const int64_t chunks = offset_at(p.ends, 0, p.q_tokens) * CHUNKS;
+    for (int64_t i = threadIdx.x; i < chunks; i += 64 * kWaves)
+      *reinterpret_cast<u32x4_t*>(p.out + (i / CHUNKS * p.heads + head) * D + i % CHUNKS * 8) =
+          u32x4_t{0u, 0u, 0u, 0u};
+    return;
+  }
+  --index;
+
   // The block's rows; true if some result is NaN or infinite.  Two copies of the
   // code, so that the second pass costs the first no registers.
   auto attend = [&](auto second, int lane) __attribute__((always_inline)) -> bool {
@@ -463,7 +474,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
 
 int launch_prompt_attention(const PromptParams& p, int dtype, hipStream_t st) {
   auto go = [&](auto kernel) -> int {
-    const int64_t blocks = ((p.q_tokens + kBlockRows - 1) / kBlockRows + p.seqs) * p.heads;
+    // a partial block for every sequence and for the rows behind them, one for the rows in front
+    const int64_t blocks = ((p.q_tokens + kBlockRows - 1) / kBlockRows + p.seqs + 1) * p.heads;
     if (blocks > INT32_MAX) return GRINQH_ERR_INVALID;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * kWaves), 0, st, p);
     return hipGetLastError() == hipSuccess ? GRINQH_OK : GRINQH_ERR_HIP;

@@ -179,8 +179,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
     """Causal attention over packed sequences: ``q [tokens, heads, head_dim]``, ``k`` and ``v [keys, kv_heads,
     head_dim]``.  Sequence s has rows ``ends[s] .. ends[s + 1] - 1`` (int32 ``[seqs + 1]``, ascending) and keys
     ``key_ends[s] .. key_ends[s + 1] - 1`` (default: as its rows); its last row sees all its keys, the row before one
-    fewer, and so on.  Rows that see no key, or lie behind the last sequence, give zeros.  ``scale`` defaults to
-    head_dim ** -0.5."""
+    fewer, and so on.  Rows that see no key, or lie in front of the first sequence or behind the last, give zeros.
+    ``scale`` defaults to head_dim ** -0.5."""
     dev, dtype = q.device, q.dtype
     if not q.is_cuda:
         raise ValueError(f"GRINQH: q must be on a HIP device (got {dev}); there is no CPU path")
