@@ -69,3 +69,47 @@ def test_prompt_rows_before_the_first_sequence(ends, heads):
     stale = torch.full((tokens, heads, 64), float("nan"), dtype=q.dtype, device="cuda")
     del stale, out
     _check_prompt(ga.prompt_attention(q, k, v, _dev(ends), _dev(key_ends)), q, k, v, ends, key_ends, "f16")
+
+
+# ---------------------------------------------------------------- layouts that the kernels cannot read in place
+
+def _odd_layouts(x):
+    """x [tokens, heads, d] where its rows are not 16-byte aligned although torch calls the tensor contiguous, and
+    one token or head with distances that do not matter"""
+    t, h, d = x.shape
+    shifted = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(t, h, d)
+    yield shifted.copy_(x)
+    if t == 1:
+        wide = torch.empty((4, h, d), dtype=x.dtype, device=x.device)
+        wide[:1] = x
+        for distance in (0, 3, (1 << 23) + 8):
+            yield wide.as_strided((1, h, d), (distance, d, 1))
+    if h == 1:
+        wide = torch.empty((t, 1, d + 1), dtype=x.dtype, device=x.device)
+        yield wide[:, :, 1:].copy_(x)
+        yield x.as_strided((t, 1, d), (d, 5, 1))
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 33])
+@pytest.mark.parametrize("heads", [1, 3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_layouts_are_copied(tokens, heads, d):
+    from grinqh import attention as ga
+    rng = np.random.default_rng(tokens)
+    q, k, v = (_randn(rng, tokens, heads, d) for _ in range(3))
+    slots = torch.arange(tokens).cuda()
+    table = torch.zeros((tokens, 3), dtype=torch.int32, device="cuda")
+    table[:, 1], table[:, 2] = 1, 2
+    lengths = torch.full((tokens,), tokens, dtype=torch.int32, device="cuda")
+    ends = _dev([0, tokens])
+    cache, again = ga.kv4_cache(3, heads, d), ga.kv4_cache(3, heads, d)
+    ga.kv4_store(cache, k, v, slots)
+    decode, prompt = ga.kv4_attention(q, cache, table, lengths), ga.prompt_attention(q, k, v, ends)
+    for k2, v2, q2 in zip(_odd_layouts(k), _odd_layouts(v), _odd_layouts(q)):
+        for a, b in ((k2, v), (k, v2)):
+            again.zero_()
+            ga.kv4_store(again, a, b, slots)
+            assert torch.equal(again, cache)
+        assert torch.equal(ga.kv4_attention(q2, cache, table, lengths), decode)
+        for args in ((q2, k, v), (q, k2, v), (q, k, v2)):
+            assert torch.equal(ga.prompt_attention(*args, ends), prompt)

@@ -72,3 +72,22 @@ def test_attention_runs_on_the_tensors_device(monkeypatch, current):
     ga._WORKSPACES._bufs.clear()
     assert devices.calls == [(f"grinqh_{n}", 1) for n in ("kv4_store", "kv4_load", "kv4_attention", "prompt_attention")]
     assert devices.current == current
+
+
+def _askew(x):
+    """x [tokens, heads, d], called contiguous by torch, one element off the alignment that the kernels read"""
+    return torch.empty(x.numel() + 1, dtype=x.dtype)[1:].view(x.shape).copy_(x)
+
+
+def test_rows_are_copied_where_the_kernels_cannot_read_them():
+    x = torch.randn((4, 3, 128)).half()
+    wide = torch.randn((4, 1, 129)).half()
+    cases = [_askew(x), _askew(x[:1]), wide[:, :, 1:], wide[:1, :, 1:], x[:1].as_strided((1, 3, 128), (3, 128, 1)),
+             x[:1].as_strided((1, 3, 128), ((1 << 23) + 8, 128, 1)), x[:, :1].as_strided((4, 1, 128), (384, 5, 1)),
+             x[:1].expand(4, -1, -1), x.as_strided((4, 3, 128), (64, 128, 1))]
+    for y in cases:
+        got, token, head = ga._rows(y, "x", y.device, y.dtype, 128)
+        assert torch.equal(got, y) and got.data_ptr() % 16 == 0 and got.stride() == (token, head, 1)
+        assert 128 <= token <= 1 << 23 and token % 8 == 0 and 0 <= head <= 1 << 23 and head % 8 == 0
+    for y in (x, x[:, :2], x[::2], x.transpose(0, 1), x[:1].expand(4, -1, -1)):  # read in place
+        assert ga._rows(y, "x", y.device, y.dtype)[0] is y

@@ -67,9 +67,10 @@ def _cache_layout(cache: torch.Tensor) -> Tuple[int, int, int, int, int]:
     return shape[0], shape[1], 16 * shape[2], layout[0], layout[1]
 
 
-def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> Tuple[torch.Tensor, int, int]:
-    """x [tokens, heads, head_dim] as the kernels read it (16-byte aligned rows, distances multiples of 8; copied
-    where it is not), and its token and head distances"""
+def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype,
+          least: int = 0) -> Tuple[torch.Tensor, int, int]:
+    """x [tokens, heads, head_dim] as the kernels read it (16-byte aligned rows, distances multiples of 8, tokens at
+    least ``least`` apart; copied where it is not), and its token and head distances"""
     if x.device != device or x.dtype is not dtype:
         raise ValueError(f"GRINQH: {name} must be {dtype} on {device}, got {x.dtype} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
@@ -78,8 +79,8 @@ def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) 
     if len(stride) != 3:
         raise ValueError(f"GRINQH: {name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
     t, h, c = stride
-    if c != 1 or t % 8 or h % 8 or t > 1 << 23 or h > 1 << 23 or x.data_ptr() % 16:
-        x = x.contiguous()
+    if c != 1 or t % 8 or h % 8 or t < least or t > 1 << 23 or h > 1 << 23 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)  # contiguous() keeps what only lies askew
         t, h, c = x.stride()
     return x, t, h
 
@@ -186,14 +187,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
         raise ValueError(f"GRINQH: q must be on a HIP device (got {dev}); there is no CPU path")
     dt = _dtype_code(dtype)
     q, q_token, q_head = _rows(q, "q", dev, dtype)
-    k, k_token, k_head = _rows(k, "k", dev, dtype)
-    v, v_token, v_head = _rows(v, "v", dev, dtype)
     tokens, heads, d = q.shape
+    k, k_token, k_head = _rows(k, "k", dev, dtype, d)  # not broadcast, not overlapping
+    v, v_token, v_head = _rows(v, "v", dev, dtype, d)
     keys, kv_heads, dk = k.shape
-    if k_token < dk:  # broadcast or overlapping rows
-        k, k_token, k_head = _rows(k.contiguous(), "k", dev, dtype)
-    if v_token < dk:
-        v, v_token, v_head = _rows(v.contiguous(), "v", dev, dtype)
     if d not in HEAD_DIMS or dk != d or v.shape != k.shape or kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"GRINQH: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit: head_dim "
                          f"must be one of {HEAD_DIMS}, the heads a multiple of the key/value heads")
