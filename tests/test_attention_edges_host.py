@@ -91,3 +91,20 @@ def test_rows_are_copied_where_the_kernels_cannot_read_them():
         assert 128 <= token <= 1 << 23 and token % 8 == 0 and 0 <= head <= 1 << 23 and head % 8 == 0
     for y in (x, x[:, :2], x[::2], x.transpose(0, 1), x[:1].expand(4, -1, -1)):  # read in place
         assert ga._rows(y, "x", y.device, y.dtype)[0] is y
+
+
+def test_tangents_are_refused():
+    """a forward-mode dual does not require a gradient; its tangent must not be dropped in silence"""
+    x = torch.randn((4, 3, 128)).half()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for y in (dual, dual[:, :2], dual[:1, 1:]):
+            with pytest.raises(ValueError, match="tangent"):
+                ga._rows(y, "q", x.device, x.dtype)
+        assert ga._rows(x, "q", x.device, x.dtype)[0] is x
+
+    def through(y):
+        with pytest.raises(ValueError, match="tangent"):
+            ga._rows(y, "q", x.device, x.dtype)
+        return y * 2
+    torch.func.jvp(through, (x,), (torch.ones_like(x),))

@@ -8,8 +8,9 @@ These functions are the middle part: ``prompt_attention`` for prompts,
 single tokens that follow and ``kv4_load`` for a later prompt that shares a
 cached prefix.  Queries, keys and values may be slices of the fused projection;
 all calls only enqueue work on the current stream and can be captured in a HIP
-graph.  There is no backward pass: inputs that require a gradient are refused
-while gradients are recorded.  No reference counterpart: the reference leaves
+graph.  There is no backward pass and no forward-mode derivative: inputs that
+require a gradient while gradients are recorded, or that carry a tangent, are
+refused.  No reference counterpart: the reference leaves
 attention to vLLM.
 """
 from __future__ import annotations
@@ -18,6 +19,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 from .kernel import _Workspaces, _dtype_code
@@ -75,6 +77,8 @@ def _rows(x: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype,
         raise ValueError(f"GRINQH: {name} must be {dtype} on {device}, got {x.dtype} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"GRINQH: {name} requires a gradient; the attention operators have no backward pass")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"GRINQH: {name} has a tangent; the attention operators have no forward-mode derivative")
     stride = x.stride()
     if len(stride) != 3:
         raise ValueError(f"GRINQH: {name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
