@@ -234,7 +234,10 @@ int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_siz
  * workspace (grinqh_kv4_attention_workspace_bytes for a capacity of table_width *
  * page_size tokens, 256-byte aligned) is zero-filled once before its first use
  * (every call leaves its counters zero again); calls that share one must be
- * ordered (same stream). */
+ * ordered (same stream).  Its size grows with seqs up to 1024 sequences and
+ * 2^15 pairs of a sequence and up to 16 query heads of one key/value head, and
+ * is 0 beyond, where no sequence is shared between blocks: one workspace for
+ * batches of many sizes is that of the largest batch within. */
 size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t capacity);
 int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
                          int64_t pages, int kv_heads, int page_size, int head_dim, int group,

@@ -113,3 +113,30 @@ def test_layouts_are_copied(tokens, heads, d):
         assert torch.equal(ga.kv4_attention(q2, cache, table, lengths), decode)
         for args in ((q2, k, v), (q, k2, v), (q, k, v2)):
             assert torch.equal(ga.prompt_attention(*args, ends), prompt)
+
+
+# ---------------------------------------------------------------- workspaces
+
+def test_largest_batch_covers_smaller_ones_in_a_capture():
+    """a batch too large to share its sequences, run once, leaves the workspace that smaller batches share theirs in"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(21)
+    cache, table, lengths, kv = _paged(rng, [3000, 40], 1, 64, 16, 64, "f16")
+    pick = torch.arange(1025).cuda() % 2
+    q = _randn(rng, 2, 2, 64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ga.kv4_attention(q[pick], cache, table[pick], lengths[pick])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = ga.kv4_attention(q, cache, table, lengths)
+    torch.cuda.synchronize()
+    for i in range(3):
+        q.copy_(_randn(rng, 2, 2, 64))
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        _check_decode(got, q, kv, 64, "f16")
+        assert torch.equal(got, ga.kv4_attention(q, cache, table, lengths))

@@ -108,3 +108,18 @@ def test_tangents_are_refused():
             ga._rows(y, "q", x.device, x.dtype)
         return y * 2
     torch.func.jvp(through, (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,capacity", [(32, 8, 128, 8192), (2, 1, 64, 2048), (64, 8, 256, 1 << 20),
+                                                       (40, 40, 64, 4096), (17, 1, 128, 1056), (128, 1, 64, 40000),
+                                                       (8, 8, 128, 1024)])
+def test_workspace_covers_all_smaller_batches(heads, kv_heads, d, capacity):
+    ga._workspace_bytes.cache_clear()
+    query = _lib.load_library().grinqh_kv4_attention_workspace_bytes
+    most = 0
+    for seqs in range(1, 4300):
+        most = max(most, query(seqs, heads, kv_heads, d, capacity))
+        assert ga._workspace_bytes(seqs, heads, kv_heads, d, capacity) == most
+    assert (most > 0) == (capacity > 1024)
+    assert ga._workspace_bytes(1 << 20, heads, kv_heads, d, capacity) == most
+    ga._workspace_bytes.cache_clear()

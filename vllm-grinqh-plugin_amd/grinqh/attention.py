@@ -54,6 +54,11 @@ def kv4_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 16, gro
                        device=device)
 
 
+# The largest batch whose sequences may be shared by several blocks, in sequences
+# and in pairs of a sequence and up to 16 query heads of one key/value head.
+_SHARED_SEQS = 1024
+_SHARED_UNITS = 1 << 15
+
 _LAYOUTS = {kv4_record_bytes(d, g): (d, g) for d in HEAD_DIMS for g in GROUPS if g <= d}
 
 
@@ -105,6 +110,11 @@ def _scale(scale: Optional[float], head_dim: int) -> float:
 
 @lru_cache(maxsize=1024)
 def _workspace_bytes(seqs: int, heads: int, kv_heads: int, head_dim: int, capacity: int) -> int:
+    """Workspace of this batch and of every smaller one, so that a program which ran its largest batch can capture the
+    others: the library's sizes grow with the batch up to the largest that may share its sequences between blocks, and
+    are 0 beyond."""
+    tiles = kv_heads * -(-(heads // kv_heads) // 16)
+    seqs = min(seqs, _SHARED_SEQS, _SHARED_UNITS // tiles) if heads >= kv_heads else seqs
     return _lib.load_library().grinqh_kv4_attention_workspace_bytes(seqs, heads, kv_heads, head_dim, capacity)
 
 
