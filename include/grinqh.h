@@ -210,7 +210,8 @@ int grinqh_gemm_or_gemv_noalloc(const void* x, int64_t M, int64_t K, int64_t ldx
  * head.  Values are limited to +-65504; minimum = f16(min), scale =
  * f16((max - minimum) / 15) (the fp32 product with 1/15), code = round((x -
  * minimum) * (1 / scale)) in 0..15, what a code stands for is minimum + scale *
- * code.  A group that holds a NaN is NaN. */
+ * code (up to 65536 where the scale was rounded up; fp16 results are limited to
+ * +-65504).  A group that holds a NaN is NaN. */
 size_t grinqh_kv4_record_bytes(int head_dim, int group);
 
 /* Writes the keys and values of `tokens` tokens at their slots (int64 [tokens],

@@ -140,3 +140,43 @@ def test_largest_batch_covers_smaller_ones_in_a_capture():
         got = out.clone()
         _check_decode(got, q, kv, 64, "f16")
         assert torch.equal(got, ga.kv4_attention(q, cache, table, lengths))
+
+
+# ---------------------------------------------------------------- magnitudes
+
+def test_values_at_the_limit_stay_finite():
+    """a scale that rounds up makes the largest code stand for more than fp16 holds: results are limited as the stored
+    values are; NaN stays NaN"""
+    from grinqh import attention as ga
+    d = 128
+    x = torch.zeros((6, 1, d), dtype=torch.float16, device="cuda")
+    x[0, 0, ::2] = LIMIT                                  # scale 4368: code 15 stands for 65520
+    x[1, 0, ::2], x[1, 0, 1::2] = LIMIT, -LIMIT           # scale 8736: code 15 stands for 65536
+    x[2, 0, 3] = float("inf")
+    x[3, 0, 5] = float("-inf")
+    x[4], x[5, 0, 7] = -LIMIT, float("nan")
+    slots = torch.arange(6).cuda()
+    cache = ga.kv4_cache(6, 1, d, 16, 32)
+    ga.kv4_store(cache, x, x, slots * 16)
+    k, v = ga.kv4_load(cache, slots * 16, torch.float16)
+    for got in (k, v):
+        assert bool(got[:5].isfinite().all()) and float(got[0].max()) == LIMIT and float(got[1].max()) == LIMIT
+        assert float(got[2].max()) == LIMIT and float(got[3].min()) == -LIMIT and bool((got[4] == -LIMIT).all())
+        assert bool(got[5, 0, :32].isnan().all())
+    wide, _ = ga.kv4_load(cache, slots * 16, torch.bfloat16)
+    assert float(wide[0].max()) == 65536.0  # the limit, and 65520, to 8 bits
+    # one key each
+    lengths = torch.ones(6, dtype=torch.int32, device="cuda")
+    q = torch.ones((6, 1, d), dtype=torch.float16, device="cuda")
+    out = ga.kv4_attention(q, cache, slots.int().view(6, 1), lengths)
+    assert bool(out[:5].isfinite().all()) and bool(out[5].isnan().all())
+    # a weight's rounding (2^-11) times what is left of 15 codes about their middle, and the result's own rounding
+    scale = torch.tensor([4368.0, 8736.0, 4368.0, 4368.0, 0.0], device="cuda").view(5, 1, 1)
+    assert bool(((out[:5].float() - v[:5].float()).abs() <= 2.0 ** -11 * (7.5 * scale + v[:5].float().abs())).all())
+    # many equal keys, joined over several blocks
+    cache = ga.kv4_cache(200, 1, d, 16)
+    t = torch.arange(3000).cuda()
+    ga.kv4_store(cache, x[:1].expand(3000, -1, -1), x[1:2].expand(3000, -1, -1), t)
+    q = torch.ones((1, 2, d), dtype=torch.float16, device="cuda")
+    out = ga.kv4_attention(q, cache, torch.arange(200).int().cuda().view(1, -1), torch.tensor([3000]).int().cuda())
+    assert bool(out.isfinite().all()) and bool((out.float().abs() >= LIMIT * (1 - 2.0 ** -9)).all())

@@ -43,6 +43,16 @@ __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
 __device__ __forceinline__ float half_lo(uint32_t w) { return f16_bits_to_f32((uint16_t)w); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return f16_bits_to_f32((uint16_t)(w >> 16)); }
 
+// What is kept is within +-kLimit, but a scale that was rounded up makes the
+// largest code stand for up to 65536, and weights round too: fp16 results are
+// limited, as they would be infinite otherwise (bf16 holds 65536).  NaN stays.
+template <typename DT>
+__device__ __forceinline__ uint16_t limited(float v) {
+  if constexpr (DT::id == F16::id)
+    v = __builtin_elementwise_maximum(__builtin_elementwise_minimum(v, kLimit), -kLimit);
+  return from_f32<DT>(v);
+}
+
 // ---------------------------------------------------------------- store, load
 
 // The value of the lane that DPP control `CTRL` names.
@@ -145,7 +155,7 @@ __device__ __forceinline__ u32x4_t dequantize8(uint32_t w, uint32_t params) {
   for (int p = 0; p < 4; ++p) {
     const float a = fmaf(s, (float)((w >> (4 * p)) & 15u), m);
     const float b = fmaf(s, (float)((w >> (4 * p + 16)) & 15u), m);
-    out[p] = (uint32_t)from_f32<DT>(a) | ((uint32_t)from_f32<DT>(b) << 16);
+    out[p] = (uint32_t)limited<DT>(a) | ((uint32_t)limited<DT>(b) << 16);
   }
   return out;
 }
@@ -620,7 +630,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
       val = fmaf(f, sh.o[w][row][d] + s_off[w][row], val);
     }
     if (share.runs == 1) {
-      p.out[out_row * D + at] = from_f32<DT>(length > 0 || sum != sum ? val / sum : 0.f);
+      p.out[out_row * D + at] = limited<DT>(length > 0 || sum != sum ? val / sum : 0.f);
     } else {
       store_partial(slot + at, val);
       if (d == 0) {
@@ -711,8 +721,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
     if (live && part == 0) {
       const float inv = 1.f / s_l[0][row];
       *reinterpret_cast<u32x2_t*>(p.out + out_row * D + 4 * column) =
-          u32x2_t{(uint32_t)from_f32<DT>(val[0] * inv) | ((uint32_t)from_f32<DT>(val[1] * inv) << 16),
-                  (uint32_t)from_f32<DT>(val[2] * inv) | ((uint32_t)from_f32<DT>(val[3] * inv) << 16)};
+          u32x2_t{(uint32_t)limited<DT>(val[0] * inv) | ((uint32_t)limited<DT>(val[1] * inv) << 16),
+                  (uint32_t)limited<DT>(val[2] * inv) | ((uint32_t)limited<DT>(val[3] * inv) << 16)};
     }
   }
   if (threadIdx.x == 0) atomicExch(&p.counters[unit], 0u);
