@@ -252,7 +252,8 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
  * when that is negative (zeros).  Rows in front of the first sequence (q_ends[0]
  * > 0) and behind the last give zeros.
  * Keys and values that a row does not see have no effect on it, whatever they
- * hold.  Offsets are limited to the tensors.  k_token and v_token are at least
+ * hold; an infinite value that it sees makes its channel infinite (NaN with one
+ * of the other sign), whatever its weight.  Offsets are limited to the tensors.  k_token and v_token are at least
  * head_dim; scale > 0. */
 int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                             int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const int32_t* q_ends,

@@ -51,6 +51,23 @@ def test_prompt_later_values_do_not_count(dtype, d, rows, keys):
     assert torch.equal(out.nan_to_num(0.0, inf, -inf), want.nan_to_num(0.0, inf, -inf))
 
 
+def test_prompt_infinite_values_of_small_weight():
+    """an infinite value counts for the rows that see it also where its weight rounds to zero in fp16"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(77)
+    n, key, inf = 400, 150, float("inf")
+    q, k = (torch.zeros((n, 2, 128), dtype=torch.float16, device="cuda") for _ in (0, 1))
+    q[:, :, 0], k[:, :, 0], k[0, :, 0] = 16.0, -20.0, 0.0  # exp(-20) and the first key
+    v = _randn(rng, n, 2, 128)
+    want = ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.0 / 16)
+    v[key, 0, 3], v[key, 1, 7], v[key + 100, 1, 7] = inf, inf, -inf
+    out = ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.0 / 16)
+    want[key:, 0, 3], want[key:key + 100, 1, 7] = inf, inf
+    assert bool(out[key + 100:, 1, 7].isnan().all())
+    out[key + 100:, 1, 7] = want[key + 100:, 1, 7] = 0.0
+    assert torch.equal(out, want)
+
+
 # ---------------------------------------------------------------- rows of no sequence
 
 @pytest.mark.parametrize("ends", [[9, 40, 70], [300, 300, 333], [77], [200, 201], [1, 80, 80]])

@@ -344,11 +344,11 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     };
 
     // A value that is NaN or infinite must not reach the rows that do not see its
-    // key, but their weight of zero times it is NaN.  Such results send the block
-    // through its keys a second time (so do rows that see one): with `apart`, tiles
-    // that not all rows see whole are stripped of these values, which keep their
-    // place in s_first: key j is seen by the rows from j - shift on, so that the
-    // first key of each kind and channel decides.
+    // key, but their weight of zero times it is NaN; and a row that sees it must not
+    // get NaN for an infinity because its weight rounds to zero.  Such results send
+    // the block through its keys a second time: with APART the tiles are stripped of
+    // these values, which keep their place in s_first: key j is seen by the rows from
+    // j - shift on, so that the first key of each kind and channel decides.
     auto strip = [&](uint8_t* vt, int tile) {
       constexpr uint32_t kInf = DT::id == F16::id ? 0x7C00u : 0x7F80u;
       int at = 64 * wave + lane;
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     auto turn = [&](int j, uint8_t* k, uint8_t* v, uint8_t* v_next) {
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
-      if (APART && j * kKeys + kKeys - 1 > (int)block * kBlockRows + shift) {
+      if constexpr (APART) {
         strip(v, j);
         __syncthreads();
       }
