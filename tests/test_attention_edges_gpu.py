@@ -197,3 +197,26 @@ def test_values_at_the_limit_stay_finite():
     q = torch.ones((1, 2, d), dtype=torch.float16, device="cuda")
     out = ga.kv4_attention(q, cache, torch.arange(200).int().cuda().view(1, -1), torch.tensor([3000]).int().cuda())
     assert bool(out.isfinite().all()) and bool((out.float().abs() >= LIMIT * (1 - 2.0 ** -9)).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_values_at_the_limit_stay_finite(d):
+    """fp16 weights are rounded and their sum is not, so that a mean of values at the limit may come out above it: one
+    key of the second tile has nearly all the weight, which is not a power of two as the reference is the first key's"""
+    from grinqh import attention as ga
+    n, key = 400, 70
+    q, k = (torch.zeros((n, 2, d), dtype=torch.float16, device="cuda") for _ in (0, 1))
+    q[:, :, 0] = 16.0
+    q[:, :, 1] = torch.linspace(3.0, 5.4, n).cuda().half().view(n, 1)
+    k[:, :, 0] = -20.0
+    k[0, :, 0], k[key, :, 0], k[key, :, 1] = 0.0, 0.0, 16.0
+    v = torch.full((n, 2, d), LIMIT, dtype=torch.float16, device="cuda")
+    v[:, :, 1::2] = -LIMIT
+    out = ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.0 / 16)
+    assert bool(out.isfinite().all())
+    _check_prompt(out, q, k, v, [0, n], [0, n], "f16", 1.0 / 16)
+    seen, inf = 150, float("inf")  # infinities are no such excess
+    v[seen, 1, 2], v[seen, 1, 3], v[key, 0, 5] = inf, -inf, -inf
+    again = ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.0 / 16)
+    out[seen:, 1, 2], out[seen:, 1, 3], out[key:, 0, 5] = inf, -inf, -inf
+    assert torch.equal(again, out)

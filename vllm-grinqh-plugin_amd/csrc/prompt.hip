@@ -50,6 +50,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return f32x2_to_bf16x2(lo, hi);
 }
 
+// Two results.  Weights are rounded for the second product and their sum is not,
+// so that a mean of fp16 values next to the limit may pass it: it is limited.
+// (What infinite and NaN accumulators become is put right in the second pass.)
+template <typename DT>
+__device__ __forceinline__ uint32_t pack_results(float lo, float hi) {
+  const uint32_t w = pack2<DT>(lo, hi);
+  if constexpr (DT::id != F16::id) return w;
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  const f16x2_t most = (f16x2_t)((_Float16)65504.f);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(
+                                          __builtin_elementwise_min(__builtin_bit_cast(f16x2_t, w), most), -most));
+}
+
 constexpr int kWaves = 4;
 constexpr int kBlockRows = 32 * kWaves;
 constexpr int kKeys = 64;       // keys per tile
@@ -436,7 +449,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         u32x2_t w =
-            u32x2_t{pack2<DT>(O[m][e] * inv, O[m][e + 1] * inv), pack2<DT>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
+            u32x2_t{pack_results<DT>(O[m][e] * inv, O[m][e + 1] * inv),
+                    pack_results<DT>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           odd = fmaf(O[m][e + i], 0.f, odd);
@@ -444,11 +458,12 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
             const int channel = 32 * m + 2 * e + 4 * half + i, seen = row + shift;
             const bool nan = s_first[0][channel] <= seen, up = s_first[1][channel] <= seen,
                        down = s_first[2][channel] <= seen;
-            float x = to_f32<DT>((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+            const bool finite = fabsf(O[m][e + i]) < __builtin_inff();
+            float x = finite ? to_f32<DT>((uint16_t)(w[i >> 1] >> (16 * (i & 1)))) : O[m][e + i] * inv;
             if (up) x += __builtin_inff();
             if (down) x -= __builtin_inff();
             if (nan) x = __builtin_nanf("");
-            if (nan || up || down)
+            if (!finite || nan || up || down)
               w[i >> 1] = i & 1 ? (w[i >> 1] & 0xFFFFu) | ((uint32_t)from_f32<DT>(x) << 16)
                                 : (w[i >> 1] & 0xFFFF0000u) | from_f32<DT>(x);
           }
