@@ -220,3 +220,37 @@ def test_prompt_values_at_the_limit_stay_finite(d):
     again = ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.0 / 16)
     out[seen:, 1, 2], out[seen:, 1, 3], out[key:, 0, 5] = inf, -inf, -inf
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_far_negative_logits(d):
+    """logits of -10^33 and below, all a row has: the largest takes the weight"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(d)
+    n = 150
+    q = torch.full((n, 2, d), 2.0 ** 56, dtype=torch.bfloat16, device="cuda")
+    k = (-2.0 ** 50 * torch.arange(100, 100 + n).cuda()).view(n, 1, 1).expand(n, 1, d).bfloat16()  # 8 bits each
+    v = _randn(rng, n, 1, d, dtype="bf16")
+    out = ga.prompt_attention(q, k, v, _dev([0, n]))
+    assert torch.equal(out, v[:1].expand(n, 2, d))
+    out = ga.prompt_attention(-q, k, v, _dev([0, n]))
+    assert torch.equal(out, v.expand(n, 2, d))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_large_logits_of_few_bits(d, dtype):
+    """logits around +-2^30, where fp32 steps by 64: they are sums of 16-bit integers' products here, exact in fp32, and
+    tell keys apart by more than that, so that the largest key, or several equal ones, takes all weight"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(d)
+    n = 300
+    size = 2.0 ** 14
+    k = torch.zeros((n, 2, d), device="cuda")
+    steps = torch.from_numpy(rng.permutation(np.repeat(np.arange(n // 2), 2))).cuda().float()
+    k[:, 0, 0] = size * (64 + steps % 64)
+    k[:, 1, 1] = -size * (64 + steps % 64)
+    k = (k / 64).to(DT[dtype])
+    q = torch.full((n, 4, d), size, dtype=DT[dtype], device="cuda")
+    v = _randn(rng, n, 2, d, dtype=dtype)
+    _check_prompt(ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.3), q, k, v, [0, n], [0, n], dtype, 1.3)

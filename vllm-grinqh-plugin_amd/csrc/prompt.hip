@@ -17,6 +17,7 @@
 // between the register files).  One sequence of 8192 rows, 32 heads: 528 us, 1040
 // TFLOP/s, where a library product of 8192^3 reaches 1400.  Heads of 256 channels
 // need 440 registers, one wave per SIMD: 490 TFLOP/s.
+#include <cfloat>
 #include <type_traits>
 
 #include "attention_launch.h"
@@ -66,7 +67,9 @@ __device__ __forceinline__ uint32_t pack_results(float lo, float hi) {
 constexpr int kWaves = 4;
 constexpr int kBlockRows = 32 * kWaves;
 constexpr int kKeys = 64;       // keys per tile
-constexpr float kLow = -1e30f;  // running reference before the first key (finite: -inf - -inf would be NaN)
+// running reference before the first key (finite: -inf - -inf would be NaN; a row of
+// logits below it is one for the second pass)
+constexpr float kLow = -1e30f;
 
 // A value that all lanes agree on, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -189,14 +192,16 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
   }
   --index;
 
-  // The block's rows; true if some result is NaN or infinite.  Two copies of the
-  // code, so that the second pass costs the first no registers.
-  auto attend = [&](auto second, int lane) __attribute__((always_inline)) -> bool {
+  // The block's rows, and what the second pass has to put right: values that are
+  // NaN or infinite (kApart), logits too large for the weights' arithmetic (kFar).
+  // Two copies of the code, so that the second pass costs the first no registers.
+  constexpr int kApart = 1, kFar = 2;
+  auto attend = [&](auto second, int lane, bool far) __attribute__((always_inline)) -> int {
     constexpr bool APART = decltype(second)::value;
     const int n = lane & 31, half = lane >> 5;
     Sequence sq;
     int64_t block;
-    if (find_block(p, index, lane, sq, block) < 0) return false;
+    if (find_block(p, index, lane, sq, block) < 0) return 0;
     sq = {uniform(sq.row0), uniform(sq.key0), uniform(sq.rows), uniform(sq.keys)};
     block = uniform(block);
     const int kvh = head / (p.heads / p.kv_heads);
@@ -244,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     };
 
     f32x16_t O[MT];
-    float M = kLow, sum = 0.f;
+    float M = APART && far ? -FLT_MAX : kLow, sum = 0.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m) O[m] = (f32x16_t)(0.f);
     const float c2 = p.scale * 1.44269504088896f;
@@ -277,10 +282,14 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
       return a;
     };
     u32x4_t P[4];
+    // The exponent of a weight.  S c2 is exact in here and M is not, which is the same
+    // factor for all keys of a row, but of more than 2^16 for logits past 2^28: with
+    // `far` M is in S's unit, and the difference is taken first.
+    auto power = [&](float s) { return APART && far ? (s - M) * c2 : fmaf(s, c2, -M); };
     // weights of two keys: pair q of key block b
     auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], c2, -M));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], c2, -M));
+      const float p0 = __builtin_amdgcn_exp2f(power(S[b][2 * q]));
+      const float p1 = __builtin_amdgcn_exp2f(power(S[b][2 * q + 1]));
       sum += p0 + p1;
       P[2 * b + (q >> 2)][q & 3] = pack2<DT>(p0, p1);
     };
@@ -300,10 +309,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
             top = fmaxf(top, S[b][e]);
           }
       }
-      if (__any(fmaf(top, c2, -M) > 8.f)) {
-        float m = fmaxf(M, top * c2);
+      if (__any(power(top) > 8.f)) {
+        float m = fmaxf(M, APART && far ? top : top * c2);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float f = __builtin_amdgcn_exp2f(M - m);
+        const float f = __builtin_amdgcn_exp2f(APART && far ? (M - m) * c2 : M - m);
         M = m;
         sum *= f;
 #pragma unroll
@@ -470,19 +479,24 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
         }
         if (row < rows) *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) = w;
       }
-    if (APART || tiles == 0) return false;
-    const int mine = __any(odd != odd);
+    if (APART || tiles == 0) return 0;
+    // A row's largest weight is 1 or more, where its exponent was right.
+    const bool lost = l < 0.5f && row < rows && row + shift >= 0;
+    int mine = 0;
+    if (__any(odd != odd || lost)) mine = __any(lost || fabsf(M) > 0x1p24f && M != kLow) ? kApart | kFar : kApart;
     if (lane == 0) s_redo[wave] = mine;
     __syncthreads();
     int redo = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) redo |= s_redo[w];
-    return redo != 0;
+    return redo;
   };
-  if (!attend(std::false_type{}, threadIdx.x & 63)) return;
+  const int redo = attend(std::false_type{}, threadIdx.x & 63, false);
+  if (redo == 0) return;
   int none = 0;
   asm volatile("" : "+s"(index), "+s"(head), "+s"(none));  // nothing is kept from the first pass
-  attend(std::true_type{}, __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)));
+  attend(std::true_type{}, __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)),
+         (__builtin_amdgcn_readfirstlane(redo) & kFar) != 0);
 }
 
 }  // namespace
