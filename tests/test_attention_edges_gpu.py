@@ -254,3 +254,53 @@ def test_prompt_large_logits_of_few_bits(d, dtype):
     q = torch.full((n, 4, d), size, dtype=DT[dtype], device="cuda")
     v = _randn(rng, n, 2, d, dtype=dtype)
     _check_prompt(ga.prompt_attention(q, k, v, _dev([0, n]), scale=1.3), q, k, v, [0, n], [0, n], dtype, 1.3)
+
+
+@pytest.mark.parametrize("tokens", [5, 40, 3000])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_decode_far_logits(tokens, d):
+    """logits of -10^33 and 10^34: the largest, or all that bf16 rounds to it, take the weight"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(tokens + d)
+    cache = ga.kv4_cache(190, 1, d)
+    t = torch.arange(tokens).cuda()
+    k = torch.linspace(100.0, 1000.0, tokens).cuda().view(-1, 1, 1).expand(tokens, 1, d).bfloat16()
+    v = _randn(rng, tokens, 1, d, dtype="bf16")
+    ga.kv4_store(cache, k, v, t)
+    _, kept = ga.kv4_load(cache, t, torch.bfloat16)
+    table, lengths = torch.arange(190).int().cuda().view(1, -1), torch.tensor([tokens]).int().cuda()
+    q = torch.full((1, 2, d), 1e31, dtype=torch.bfloat16, device="cuda")
+    for sign, same in ((-1.0, k[:, 0, 0] == k[0, 0, 0]), (1.0, k[:, 0, 0] == k[-1, 0, 0])):
+        out = ga.kv4_attention(sign * q, cache, table, lengths)
+        want = kept[same].double()
+        # a weight's rounding times the codes about their middle; two roundings to bf16
+        step = (want.amax(-1) - want.amin(-1)).max() / 15
+        tol = 2.0 ** -11 * 7.5 * step + 2.0 ** -7 * want.abs().mean(0)
+        assert bool(((out.double() - want.mean(0)).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens", [40, 3000])
+def test_decode_large_logits_of_few_bits(tokens, dtype):
+    """logits around +-2^36, exact in fp32 (codes 0 to 15 of one scale, a power of two), that tell tokens apart by more
+    than fp32's step there"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(tokens)
+    d, sign = 64, torch.tensor([1.0, -1.0], device="cuda")
+    code = torch.from_numpy(rng.integers(0, 16, tokens)).cuda()
+    k = torch.zeros((tokens, 1, d), device="cuda")
+    k[:, :, 0::2], k[:, :, 1::2] = 30720.0, 0.0  # 15 * 2048
+    k[:, 0, 0] = code * 2048.0
+    k, v = k.to(DT[dtype]), _randn(rng, tokens, 1, d, dtype=dtype)
+    cache = ga.kv4_cache(190, 1, d)
+    t = torch.arange(tokens).cuda()
+    ga.kv4_store(cache, k, v, t)
+    _, kept = ga.kv4_load(cache, t, torch.bfloat16)
+    q = torch.zeros((1, 2, d), dtype=DT[dtype], device="cuda")
+    q[0, :, 0] = sign.to(q.dtype) * 2.0 ** 14
+    q[0, :, 2] = 3 * 2.0 ** 14
+    out = ga.kv4_attention(q, cache, torch.arange(190).int().cuda().view(1, -1), torch.tensor([tokens]).int().cuda(),
+                           scale=1.3)
+    for head, best in ((0, code.max()), (1, code.min())):
+        want = kept[code == best].double().mean(0)[0]
+        assert float((out[0, head].double() - want).abs().max()) <= 2.0 ** -7 * float(kept.abs().max())

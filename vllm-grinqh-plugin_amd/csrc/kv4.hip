@@ -21,6 +21,7 @@
 // 16-byte load.  Masking a word with 0x000F000F gives two codes as fp16
 // subnormals c * 2^-24 (exact), with 0x00F000F0 two more as 16 c * 2^-24: 5 VALU
 // operations unpack 8 key codes, 6 unpack 8 value codes, and nothing is rounded.
+#include <cfloat>
 #include <type_traits>
 
 #include "attention_launch.h"
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Cache cache, const int
 constexpr int kRows = 16;       // query heads of one key/value head per block
 constexpr int kGroup = 16;     // sequences a lane looks at: plans cover 64 of these
 constexpr int kRuns = 256;      // most blocks that share one sequence and head
-constexpr float kLow = -1e30f;  // running reference before the first token (finite: -inf - -inf would be NaN)
+constexpr float kLow = -FLT_MAX;  // running reference before the first token (finite: -inf - -inf would be NaN)
 
 // Which run of 32-token steps a block takes.
 struct Share {
@@ -454,6 +455,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
 #pragma unroll
     for (int j = 0; j < ACCS; ++j) O[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float M = kLow, L = 0.f, off = 0.f;
+  float zs = qs;  // unit of the logits z
+  bool far = false;
 
   auto compute = [&](const Tokens<D, G>& t, int step) {
 #pragma unroll
@@ -493,10 +496,20 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
     }
     __builtin_amdgcn_sched_barrier(0);  // keys, weights, values: unpacking ahead would not fit the registers
     float pe[8], pw[8];
+    // z qs is exact in here and M is not: the same factor for all tokens of a row, but
+    // of more than 2^16 for logits past 2^28.  With `far` the product is rounded first.
+    auto product_first = [&]() {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z[e] *= qs;
+        asm volatile("" : "+v"(z[e]));  // not contracted with the subtraction
+      }
+    };
+    if (far) product_first();
     auto weights = [&]() {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        pe[e] = __builtin_amdgcn_exp2f(fmaf(z[e], qs, -M));
+        pe[e] = __builtin_amdgcn_exp2f(fmaf(z[e], zs, -M));
         pw[e] = fmaf(pe[e], half_lo(vp[e >> 2][e & 3]), 0.f);  // + 0: one v_fma_mix_f32, no conversion
       }
     };
@@ -514,12 +527,22 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
     const bool raise = __any(top > 256.f || sum > 0x1p60f);
     float f = 1.f;
     if (raise) {
-      float m = M;
+      float m;
+      auto reach = [&]() {
+        m = M;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        m = fmaxf(m, fmaf(z[e], qs, __log2f(fmaxf(half_lo(vp[e >> 2][e & 3]), 0x1p-24f))));
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
+        for (int e = 0; e < 8; ++e)
+          m = fmaxf(m, fmaf(z[e], zs, __log2f(fmaxf(half_lo(vp[e >> 2][e & 3]), 0x1p-24f))));
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+      };
+      reach();
+      if (!far && __any(fabsf(m) > 0x1p24f && m != kLow)) {
+        far = true;
+        zs = 1.f;
+        product_first();
+        reach();
+      }
       f = __builtin_amdgcn_exp2f(M - m);
       M = m;
       L *= f;
