@@ -304,3 +304,21 @@ def test_decode_large_logits_of_few_bits(tokens, dtype):
     for head, best in ((0, code.max()), (1, code.min())):
         want = kept[code == best].double().mean(0)[0]
         assert float((out[0, head].double() - want).abs().max()) <= 2.0 ** -7 * float(kept.abs().max())
+
+
+@pytest.mark.parametrize("tokens", [5, 40, 3000])
+@pytest.mark.parametrize("size,scale", [(2.0 ** 120, None), (1e-25, 1e-25), (2.0 ** 127, 1e3), (1e-38, 1e-37)])
+def test_decode_queries_of_any_size(tokens, size, scale):
+    """queries and scales whose product with the codes' unit leaves fp32's range, equal logits: the mean of all values"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(tokens)
+    d = 128
+    cache = ga.kv4_cache(190, 1, d)
+    t = torch.arange(tokens).cuda()
+    v = _randn(rng, tokens, 1, d, dtype="bf16")
+    ga.kv4_store(cache, torch.zeros_like(v), v, t)
+    _, kept = ga.kv4_load(cache, t, torch.bfloat16)
+    table, lengths = torch.arange(190).int().cuda().view(1, -1), torch.tensor([tokens]).int().cuda()
+    q = torch.full((1, 2, d), size, dtype=torch.bfloat16, device="cuda")
+    out = ga.kv4_attention(q, cache, table, lengths, scale=scale)
+    assert float((out.double() - kept.double().mean(0)).abs().max()) <= 2.0 ** -7 * float(kept.abs().max())

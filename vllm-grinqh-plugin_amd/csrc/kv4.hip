@@ -446,7 +446,9 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
       qsum[g] += __shfl_xor(qsum[g], 32, 64);
       qsum[g] *= 0x1p-24f;  // the codes' unit
     }
-    qs = ldexpf(p.scale * 1.44269504088896f, 24 - ex);  // logits in powers of two
+    // logits in powers of two; never 0 or infinite, which times an infinite or a zero
+    // logit (a token past the end, a key of zeros) would be NaN
+    qs = fminf(fmaxf(ldexpf(p.scale * 1.44269504088896f, 24 - ex), FLT_MIN), FLT_MAX);
   }
 
   f32x4_t O[M_TILES][ACCS];
