@@ -322,3 +322,16 @@ def test_decode_queries_of_any_size(tokens, size, scale):
     q = torch.full((1, 2, d), size, dtype=torch.bfloat16, device="cuda")
     out = ga.kv4_attention(q, cache, table, lengths, scale=scale)
     assert float((out.double() - kept.double().mean(0)).abs().max()) <= 2.0 ** -7 * float(kept.abs().max())
+
+
+# ---------------------------------------------------------------- refusals
+
+def test_refuses_caches_without_heads():
+    from grinqh import attention as ga
+    cache = torch.zeros((2, 0, 1, 2176), dtype=torch.uint8, device="cuda")
+    q = torch.ones((1, 4, 128), dtype=torch.float16, device="cuda")
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    for call in (lambda: ga.kv4_attention(q, cache, one.view(1, 1), one), lambda: ga.kv4_load(cache, one.long()),
+                 lambda: ga.kv4_store(cache, q[:, :0], q[:, :0], one.long())):
+        with pytest.raises(ValueError):
+            call()

@@ -68,8 +68,8 @@ def _cache_layout(cache: torch.Tensor) -> Tuple[int, int, int, int, int]:
         raise ValueError("GRINQH: the cache must be on a HIP device; there is no CPU path")
     shape = cache.shape
     layout = _LAYOUTS.get(shape[3]) if len(shape) == 4 else None
-    if layout is None or cache.dtype is not torch.uint8 or not cache.is_contiguous():
-        raise ValueError("GRINQH: a cache is a contiguous uint8 tensor [pages, kv_heads, page_size / 16, record] "
+    if layout is None or shape[1] == 0 or cache.dtype is not torch.uint8 or not cache.is_contiguous():
+        raise ValueError("GRINQH: a cache is a contiguous uint8 tensor [pages, kv_heads > 0, page_size / 16, record] "
                          f"(kv4_cache), got {cache.dtype} {tuple(shape)}")
     return shape[0], shape[1], 16 * shape[2], layout[0], layout[1]
 
