@@ -335,3 +335,66 @@ def test_refuses_caches_without_heads():
                  lambda: ga.kv4_store(cache, q[:, :0], q[:, :0], one.long())):
         with pytest.raises(ValueError):
             call()
+
+
+# ---------------------------------------------------------------- sequences shared by many blocks
+
+@pytest.mark.parametrize("d,per", [(64, 3), (64, 16), (128, 5), (128, 7), (128, 16), (256, 1), (256, 3), (256, 7),
+                                   (256, 12), (256, 16), (256, 17)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_decode_join(d, per, dtype):
+    """runs joined where the columns of a run are fewer than a block's threads, do not divide them, or exceed them"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(d + per)
+    lens = [5000, 33, 2049]
+    cache, table, lengths, kv = _paged(rng, lens, 1, d, 32, 64, dtype)
+    q = _randn(rng, len(lens), per, d, dtype=dtype)
+    for _ in range(2):  # the counters are zero again after a call
+        _check_decode(ga.kv4_attention(q, cache, table, lengths), q, kv, 64, dtype)
+
+
+@pytest.mark.parametrize("d,per", [(64, 2), (128, 5), (256, 16)])
+def test_decode_join_many_runs(d, per):
+    """more than 64 runs of one sequence, and more than one round of loads of them"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(d)
+    cache, table, lengths, kv = _paged(rng, [75001], 1, d, 64, d, "f16")
+    q = _randn(rng, 1, per, d)
+    _check_decode(ga.kv4_attention(q, cache, table, lengths), q, kv, d, "f16")
+
+
+@pytest.mark.parametrize("d,per", [(64, 12), (128, 9), (128, 16), (256, 5), (256, 11)])
+def test_decode_join_many_units(d, per):
+    """past 256 units the blocks have 4 waves: long sequences among them are shared all the same"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(d + per)
+    lens = rng.integers(0, 40, 140)
+    lens[[3, 70, 139]] = 6000, 1500, 20000
+    cache, table, lengths, kv = _paged(rng, lens.tolist(), 2, d, 16, 64, "bf16")
+    q = _randn(rng, len(lens), 2 * per, d, dtype="bf16")
+    _check_decode(ga.kv4_attention(q, cache, table, lengths), q, kv, 64, "bf16")
+
+
+# ---------------------------------------------------------------- inside torch.compile
+
+def test_compiled_caller():
+    """a compiled function around the calls breaks its graph at them and gives what it gives uncompiled"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(31)
+    cache, table, lengths, kv = _paged(rng, [3000, 40], 2, 64, 16, 64, "f16")
+    x, ends = _randn(rng, 90, 8, 64), _dev([0, 30, 90])
+    slots = torch.arange(90).cuda() - 1
+    fresh = ga.kv4_cache(8, 2, 64)
+
+    def layer(x, q):
+        y = x * 0.5
+        a = ga.prompt_attention(y[:, :4], y[:, 4:6], y[:, 6:], ends) + 1.0
+        ga.kv4_store(fresh, y[:, 4:6], y[:, 6:], slots)
+        k, v = ga.kv4_load(fresh, slots)
+        return a, k + 1.0, v + 1.0, ga.kv4_attention(q + 1.0, cache, table, lengths) * 2.0
+
+    compiled = torch.compile(layer, backend="eager")
+    for i in range(3):
+        q = _randn(rng, 2, 4, 64)
+        for a, b in zip(compiled(x + i, q), layer(x + i, q)):
+            assert torch.equal(a, b)
