@@ -78,9 +78,10 @@ __device__ __forceinline__ float group_reduce(float v, F&& op) {
 // of a group share the parameters.  A NaN becomes +inf in the maximum, which
 // the limit keeps finite inputs from, and makes the group's parameters NaN.
 // Channels past the limit need no limiting of their own: their codes do it.
-// VALU bound for long prompts (16 values per lane, some ten operations each):
-// 8192 tokens of 8 heads of 128 channels take 12.7 us to store (43 MB, 3.4 TB/s)
-// and 8.1 to load (5.3 TB/s).
+// Storing 8192 tokens of 8 heads of 128 channels takes 12.0 us (43 MB, 3.6 TB/s; the
+// copy rate would be 9): a lane waits for its slot before its rows leave, and of
+// its 399 VALU operations some 130 divide the slot's record by a page's (64 bits,
+// record_of).  Loading them takes 9.5 (4.6 TB/s).
 template <typename DT, int WIDTH>
 __device__ __forceinline__ uint32_t quantize8(const u32x4_t& in, uint32_t& params) {
   float x[8];
@@ -327,6 +328,8 @@ __device__ __forceinline__ void load_tokens(Tokens<D, G>& t, const uint8_t* __re
 // the same pages takes 95, the difference is the blocks' start and end.  One
 // sequence of 131072 tokens: 37 us (147 MB, 4.0 TB/s with planning and joining).
 // Short ones are latency: lengths, pages, tokens, one after the other, 8-11 us.
+// Past 1024 sequences nothing is shared (find_share): one of 32768 tokens among short
+// ones, 2 heads, takes 55 us in a batch of 1024 and 206 in one of 1025.
 //
 // S^T = K Q^T leaves a lane with one query row and 8 of the 32 tokens, which
 // is the B operand of O^T = V^T P^T: nothing crosses lanes in the loop.  With
@@ -822,7 +825,10 @@ Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t c
   // to 300 tokens, 8 heads: 10 against 16 us).
   plan.waves = units <= 256 ? 8 : 4;
   plan.blocks = plan.waves == 8 ? 256 : 512;
-  plan.least = 32;  // four rounds of 8 waves: fewer cost more in the join than they save
+  // Four rounds of 8 waves.  Of a few thousand tokens fewer would serve as well or
+  // better (1 x 4096, 8 heads: 15.2 us, 13.2 with 16 steps, 13.5 with 8; 1 x 16384 16.2,
+  // 15.8, 15.8); longer or more sequences take the same either way.
+  plan.least = 32;
   plan.slot = (per < kRows ? per : kRows) * head_size + 2 * kRows;
   // the runs beyond one per unit are at most `blocks`, and at most what the table's width allows
   const int64_t longest = (steps + plan.least - 1) / plan.least;

@@ -14,9 +14,14 @@
 // one).  One wave per SIMD issues a VALU operation every 6 cycles at most, two
 // every 4-5 (measured), so a wave has 32 rows and a SIMD two waves (64 rows and one
 // wave per SIMD would read LDS half as often, but took 826 us: accumulators moved
-// between the register files).  One sequence of 8192 rows, 32 heads: 528 us, 1040
+// between the register files).  One sequence of 8192 rows, 32 heads: 521 us, 1055
 // TFLOP/s, where a library product of 8192^3 reaches 1400.  Heads of 256 channels
-// need 440 registers, one wave per SIMD: 490 TFLOP/s.
+// need 445 registers (256 and 189 of the accumulators' file, with moves between the
+// two in the loop), one wave per SIMD: 510 TFLOP/s.
+//
+// What a first pass cannot do is left to a second one over the block's keys, which
+// blocks with NaN, infinite or very large inputs take: 2.0-2.6 times their time (3.5 with
+// heads of 256 channels).
 #include <cfloat>
 #include <type_traits>
 
@@ -286,7 +291,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     // factor for all keys of a row, but of more than 2^16 for logits past 2^28: with
     // `far` M is in S's unit, and the difference is taken first.
     auto power = [&](float s) { return APART && far ? (s - M) * c2 : fmaf(s, c2, -M); };
-    // weights of two keys: pair q of key block b
+    // Weights of two keys, pair q of key block b: in the tensors' type for the second
+    // product, the only operand it takes at that rate.  Their sum is that of the
+    // unrounded ones, so a result is off by a mean of the roundings (2^-8 and 2^-11 each
+    // at most of what they weigh, to either side).
     auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
       const float p0 = __builtin_amdgcn_exp2f(power(S[b][2 * q]));
       const float p1 = __builtin_amdgcn_exp2f(power(S[b][2 * q + 1]));
