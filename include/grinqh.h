@@ -260,6 +260,75 @@ int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, cons
                             const int32_t* k_ends, int64_t seqs, int64_t q_tokens, int64_t k_tokens, int heads,
                             int kv_heads, int head_dim, float scale, void* out, int dtype, void* stream);
 
+/* grinqh_kv4_attention with a page table per key/value head: rows of one
+ * sequence's heads are table_head apart (0: one row for all heads), so that every
+ * head can attend to pages of its own choice (grinqh_kv4_select).  All heads of a
+ * sequence have the same length; the workspace is that of grinqh_kv4_attention. */
+int grinqh_kv4_attention_selected(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads,
+                                  const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim,
+                                  int group, const int32_t* page_table, int64_t table_stride, int64_t table_head,
+                                  int table_width, const int32_t* lengths, float scale, void* out, int dtype,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Room for new tokens, from the requests' lengths, which only the device knows.
+ * Sequence s holds lengths[s] tokens and gets counts[s] more (negative ones count
+ * as 0); its rows are ends[s] .. ends[s + 1] - 1 of a buffer of `tokens` rows (less
+ * than 2^23; rows that do not fit are not granted).  Pages that it needs beyond
+ * those it has are taken from the end of free_pages[0 .. *free_count - 1], in the
+ * order of the sequences, and written into page_table (rows table_stride >=
+ * table_width apart, not overlapping).  For every row: its slot (page * page_size +
+ * place) and its position in the sequence; rows behind the last sequence, places
+ * behind the table and pages that are missing (-1 in the table, too) have slot -1.
+ * new_lengths and new_free_count hold what is left; lengths, counts, free_pages and
+ * free_count are not changed and must not overlap the results. */
+int grinqh_kv4_append(int32_t* page_table, int64_t table_stride, int table_width, int page_size,
+                      const int32_t* lengths, const int32_t* counts, int64_t seqs, const int32_t* free_pages,
+                      int64_t free_size, const int32_t* free_count, int64_t tokens, int64_t* slots, int32_t* positions,
+                      int32_t* ends, int32_t* new_lengths, int32_t* new_free_count, void* stream);
+
+/* Attention of chunks of new tokens over the cache, which holds them already:
+ * rows ends[s] .. ends[s + 1] - 1 of q (int32 [seqs + 1], ascending) attend to the
+ * first lengths[s] tokens of sequence s, the last row to all of them, the row before
+ * to one fewer, and so on.  Rows that see no token, in front of the first sequence
+ * or behind the last give zeros; a length past the table makes the sequence's
+ * results NaN, a page outside the cache those of the rows that see its tokens.
+ * Tokens that a row does not see have no effect on it.  At most 2^20 sequences;
+ * the workspace (..._workspace_bytes for a capacity of table_width * page_size
+ * tokens, 256-byte aligned) needs no initial value and holds nothing between calls. */
+size_t grinqh_kv4_chunk_attention_workspace_bytes(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_dim,
+                                                  int64_t capacity);
+int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, int64_t tokens, int heads,
+                               const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                               const int32_t* page_table, int64_t table_stride, int table_width,
+                               const int32_t* lengths, const int32_t* ends, int64_t seqs, float scale, void* out,
+                               int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The mean key of every page that tokens starts[s] .. lengths[s] - 1 of a sequence
+ * lie in (tokens in front of starts[s] in the first one counted), in 8 bits.  The
+ * summary is int8 [pages][kv_heads][head_dim + 16], 16-byte aligned: head_dim
+ * codes, their fp32 step, 12 unused bytes.  With m the mean (exact sums in 64 bits)
+ * and 2^E <= max |m| < 2^(E + 1): step = 2^(E - 6), code = round(m / step) within
+ * +-127; NaN channels count as 0, a page of zeros has step 0.  Pages outside the cache
+ * and tokens behind the table are passed over. */
+int grinqh_kv4_summarize(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                         void* summary, const int32_t* page_table, int64_t table_stride, int table_width,
+                         const int32_t* starts, const int32_t* lengths, int64_t seqs, void* stream);
+
+/* For every sequence and key/value head the `count` (at least 2) of its pages that
+ * score highest, the first and the last always among them: page indices in the
+ * order of the sequence, -1 behind the last (selected [seqs][kv_heads][count]), and
+ * how many tokens they hold (new_lengths [seqs]; a length past the table stays
+ * past the selection).  A page's score is the largest over the group's query heads of
+ * step(head) / max step * codes(head).codes(page) * step(page), the first factor at
+ * least 2^-40, where queries get codes and steps as means do (NaN as 0, infinities as
+ * the largest fp32): exact in fp32.  Equal scores: the page that comes first; a page
+ * outside the cache scores highest, so that the attention shows it. */
+size_t grinqh_kv4_select_workspace_bytes(int64_t seqs, int kv_heads, int table_width, int count);
+int grinqh_kv4_select(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* summary,
+                      int64_t pages, int kv_heads, int page_size, int head_dim, const int32_t* page_table,
+                      int64_t table_stride, int table_width, const int32_t* lengths, int count, int32_t* selected,
+                      int32_t* new_lengths, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Benchmark instrumentation; no counterpart in the reference.  Arms a one-shot
  * timer: in the next grinqh_gemm_or_gemv / grinqh_gemv_batch_union /
  * grinqh_prefill_dense call (from any thread), the dispatch of its first main

@@ -511,10 +511,15 @@ bool valid_head(int head_dim, int group) {
 bool valid_heads(int heads, int kv_heads) { return kv_heads > 0 && heads > 0 && heads % kv_heads == 0; }
 bool valid_scale(float scale) { return scale > 0.f && scale <= FLT_MAX; }
 
-bool valid_cache(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group) {
+bool valid_page(int page_size) {
   const int sub = page_size / 16;
-  if (!valid_head(head_dim, group) || kv_heads <= 0 || page_size < 16 || page_size % 16 != 0 || (sub & (sub - 1)) != 0)
-    return false;
+  return page_size >= 16 && page_size % 16 == 0 && (sub & (sub - 1)) == 0;
+}
+constexpr int64_t kMostSeqs = 1 << 20;              // of a batch, where blocks look at all of them
+constexpr int64_t kMostAppended = (1 << 23) - 1;  // sums of 256 sequences' tokens fit 32 bits
+
+bool valid_cache(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group) {
+  if (!valid_head(head_dim, group) || kv_heads <= 0 || !valid_page(page_size)) return false;
   return pages == 0 || (pages > 0 && cache != nullptr && aligned(cache, 64));
 }
 Kv4Cache kv4_cache(void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group) {
@@ -775,6 +780,16 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
                          int64_t pages, int kv_heads, int page_size, int head_dim, int group,
                          const int32_t* page_table, int64_t table_stride, int table_width, const int32_t* lengths,
                          float scale, void* out, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return grinqh_kv4_attention_selected(q, q_token, q_head, seqs, heads, cache, pages, kv_heads, page_size, head_dim,
+                                       group, page_table, table_stride, 0, table_width, lengths, scale, out, dtype,
+                                       workspace, workspace_bytes, stream);
+}
+
+int grinqh_kv4_attention_selected(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads,
+                                  const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim,
+                                  int group, const int32_t* page_table, int64_t table_stride, int64_t table_head,
+                                  int table_width, const int32_t* lengths, float scale, void* out, int dtype,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_scale(scale) || seqs < 0 || seqs > INT32_MAX ||
       !valid_cache(cache, pages, kv_heads, page_size, head_dim, group) || table_width < 0)
     return GRINQH_ERR_INVALID;
@@ -790,6 +805,7 @@ int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t
   p.sub_shift = __builtin_ctz((unsigned)p.cache.sub);
   p.table = page_table;
   p.table_stride = table_stride;
+  p.table_head = table_head;
   p.table_width = table_width;
   p.lengths = lengths;
   p.seqs = (int)seqs;
@@ -832,6 +848,145 @@ int grinqh_prompt_attention(const void* q, int64_t q_token, int64_t q_head, cons
   p.head_size = head_dim;
   p.scale = scale;
   return launch_prompt_attention(p, dtype, as_stream(stream));
+}
+
+int grinqh_kv4_append(int32_t* page_table, int64_t table_stride, int table_width, int page_size,
+                      const int32_t* lengths, const int32_t* counts, int64_t seqs, const int32_t* free_pages,
+                      int64_t free_size, const int32_t* free_count, int64_t tokens, int64_t* slots, int32_t* positions,
+                      int32_t* ends, int32_t* new_lengths, int32_t* new_free_count, void* stream) {
+  if (!valid_page(page_size) || table_width < 0 || (int64_t)table_width * page_size > INT32_MAX || seqs < 0 ||
+      seqs > kMostSeqs || free_size < 0 || free_size > INT32_MAX || tokens < 0 || tokens > kMostAppended)
+    return GRINQH_ERR_INVALID;
+  if (free_count == nullptr || ends == nullptr || new_free_count == nullptr || (free_size > 0 && free_pages == nullptr) ||
+      (tokens > 0 && (slots == nullptr || positions == nullptr)) ||
+      (seqs > 0 && (lengths == nullptr || counts == nullptr || new_lengths == nullptr ||
+                    (table_width > 0 && (page_table == nullptr || table_stride < table_width)))))
+    return GRINQH_ERR_INVALID;
+  AppendParams p;
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.page_shift = __builtin_ctz((unsigned)page_size);
+  p.lengths = lengths;
+  p.counts = counts;
+  p.seqs = (int)seqs;
+  p.free_pages = free_pages;
+  p.free_count = free_count;
+  p.free_size = (int)free_size;
+  p.tokens = (int)tokens;
+  p.slots = slots;
+  p.positions = positions;
+  p.ends = ends;
+  p.new_lengths = new_lengths;
+  p.new_free_count = new_free_count;
+  return launch_kv4_append(p, as_stream(stream));
+}
+
+size_t grinqh_kv4_chunk_attention_workspace_bytes(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_dim,
+                                                  int64_t capacity) {
+  if (tokens <= 0 || seqs < 0 || seqs > kMostSeqs || !valid_head(head_dim, head_dim) || !valid_heads(heads, kv_heads) ||
+      capacity < 0 || capacity > INT32_MAX || tokens > INT32_MAX / (heads / kv_heads))
+    return 0;
+  return plan_chunk(tokens, seqs, heads, kv_heads, head_dim, capacity).workspace;
+}
+
+int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, int64_t tokens, int heads,
+                               const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                               const int32_t* page_table, int64_t table_stride, int table_width,
+                               const int32_t* lengths, const int32_t* ends, int64_t seqs, float scale, void* out,
+                               int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_scale(scale) || seqs < 0 || seqs > kMostSeqs ||
+      tokens < 0 || tokens > INT32_MAX / (heads / kv_heads) || table_width < 0 ||
+      !valid_cache(cache, pages, kv_heads, page_size, head_dim, group))
+    return GRINQH_ERR_INVALID;
+  if (tokens == 0) return GRINQH_OK;
+  // every page index is checked against `pages`; with none there is nothing a bad one could stand for
+  if (pages == 0) table_width = 0;
+  ChunkParams p;
+  if (!head_rows(q, q_token, q_head, &p.q) || ends == nullptr || (seqs > 0 && lengths == nullptr) || out == nullptr ||
+      !aligned(out, 16) || (table_width > 0 && seqs > 0 && page_table == nullptr) ||
+      (int64_t)table_width * page_size > INT32_MAX)
+    return GRINQH_ERR_INVALID;
+  p.out = static_cast<uint16_t*>(out);
+  p.cache = kv4_cache(const_cast<void*>(cache), pages, kv_heads, page_size, head_dim, group);
+  p.sub_shift = __builtin_ctz((unsigned)p.cache.sub);
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.lengths = lengths;
+  p.ends = ends;
+  p.tokens = tokens;
+  p.seqs = (int)seqs;
+  p.heads = heads;
+  p.scale = scale;
+  p.plan = plan_chunk(tokens, seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size);
+  p.partial = static_cast<float*>(workspace);
+  if (p.plan.workspace > 0 && (workspace == nullptr || workspace_bytes < p.plan.workspace || !aligned(workspace, 256)))
+    return GRINQH_ERR_WORKSPACE;
+  return launch_chunk_attention(p, dtype, as_stream(stream));
+}
+
+int grinqh_kv4_summarize(const void* cache, int64_t pages, int kv_heads, int page_size, int head_dim, int group,
+                         void* summary, const int32_t* page_table, int64_t table_stride, int table_width,
+                         const int32_t* starts, const int32_t* lengths, int64_t seqs, void* stream) {
+  if (!valid_cache(cache, pages, kv_heads, page_size, head_dim, group) || table_width < 0 || seqs < 0 ||
+      seqs > kMostSeqs || (int64_t)table_width * page_size > INT32_MAX ||
+      (table_width > 0 && seqs > INT32_MAX / table_width / kv_heads))
+    return GRINQH_ERR_INVALID;
+  if (pages == 0 || seqs == 0 || table_width == 0) return GRINQH_OK;
+  if (summary == nullptr || !aligned(summary, 16) || page_table == nullptr || starts == nullptr || lengths == nullptr)
+    return GRINQH_ERR_INVALID;
+  SummarizeParams p;
+  p.cache = kv4_cache(const_cast<void*>(cache), pages, kv_heads, page_size, head_dim, group);
+  p.summary = static_cast<int8_t*>(summary);
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.starts = starts;
+  p.lengths = lengths;
+  p.seqs = (int)seqs;
+  p.sub_shift = __builtin_ctz((unsigned)p.cache.sub);
+  return launch_kv4_summarize(p, as_stream(stream));
+}
+
+size_t grinqh_kv4_select_workspace_bytes(int64_t seqs, int kv_heads, int table_width, int count) {
+  if (seqs <= 0 || seqs > kMostSeqs || kv_heads <= 0 || table_width <= count) return 0;
+  return (size_t)seqs * kv_heads * table_width * sizeof(float);
+}
+
+int grinqh_kv4_select(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* summary,
+                      int64_t pages, int kv_heads, int page_size, int head_dim, const int32_t* page_table,
+                      int64_t table_stride, int table_width, const int32_t* lengths, int count, int32_t* selected,
+                      int32_t* new_lengths, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype) || !valid_heads(heads, kv_heads) || !valid_head(head_dim, head_dim) || !valid_page(page_size) ||
+      seqs < 0 || seqs > kMostSeqs || pages < 0 || table_width < 0 || (int64_t)table_width * page_size > INT32_MAX ||
+      count < 2 || (int64_t)count * page_size > INT32_MAX || seqs * kv_heads > INT32_MAX)
+    return GRINQH_ERR_INVALID;
+  if (seqs == 0) return GRINQH_OK;
+  if (pages == 0) table_width = 0;  // as in grinqh_kv4_attention
+  SelectParams p;
+  if (!head_rows(q, q_token, q_head, &p.q) || lengths == nullptr || selected == nullptr || new_lengths == nullptr ||
+      (table_width > 0 && (page_table == nullptr || summary == nullptr || !aligned(summary, 16))))
+    return GRINQH_ERR_INVALID;
+  const size_t need = grinqh_kv4_select_workspace_bytes(seqs, kv_heads, table_width, count);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
+    return GRINQH_ERR_WORKSPACE;
+  p.summary = static_cast<const int8_t*>(summary);
+  p.pages = pages;
+  p.seqs = (int)seqs;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.head_size = head_dim;
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.page_shift = __builtin_ctz((unsigned)page_size);
+  p.lengths = lengths;
+  p.count = count;
+  p.scores = static_cast<float*>(workspace);
+  p.selected = selected;
+  p.new_lengths = new_lengths;
+  return launch_kv4_select(p, dtype, as_stream(stream));
 }
 
 }  // extern "C"

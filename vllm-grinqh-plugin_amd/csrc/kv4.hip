@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
   // Two slots of tokens: one is computed while the other's loads are in flight
   // (8 waves per CU then have 35 KB on their way; a third slot gave nothing).
   constexpr int SLOTS = 2;
-  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
+  const int32_t* table = p.table + (int64_t)seq * p.table_stride + (int64_t)kvh * p.table_head;
   const int last_rec = max((length - 1) >> 4, 0);
   auto record = [&](int step, int r, int page) -> const uint8_t* {
     if ((uint32_t)page >= (uint64_t)p.cache.pages) {

@@ -67,6 +67,17 @@ SIGNATURES = {
                                     _vp, ctypes.c_float, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
     "grinqh_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                        _i32, _i32, _i32, ctypes.c_float, _vp, _i32, _vp]),
+    "grinqh_kv4_attention_selected": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
+                                             _i64, _i32, _vp, ctypes.c_float, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
+    "grinqh_kv4_append": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                 _vp]),
+    "grinqh_kv4_chunk_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i32, _i32, _i32, _i64]),
+    "grinqh_kv4_chunk_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
+                                          _i32, _vp, _vp, _i64, ctypes.c_float, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
+    "grinqh_kv4_summarize": (_i32, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _vp]),
+    "grinqh_kv4_select_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32, _i32]),
+    "grinqh_kv4_select": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i32,
+                                 _vp, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
     "grinqh_time_next_product": (_i32, [_vp, _vp]),
     "grinqh_expire_tile_waits": (_i32, [_i32]),
     "grinqh_product_kernel": (_i32, [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32,

@@ -5,8 +5,11 @@ grinqh_prompt_attention).
 A decoder layer runs ``qkv_proj`` (a GRINQH linear), attention, ``o_proj``.
 These functions are the middle part: ``prompt_attention`` for prompts,
 ``kv4_store`` for the new tokens' keys and values, ``kv4_attention`` for the
-single tokens that follow and ``kv4_load`` for a later prompt that shares a
-cached prefix.  Queries, keys and values may be slices of the fused projection;
+single tokens that follow, ``kv4_chunk_attention`` for several new tokens per
+sequence behind cached ones, and ``kv4_load`` for reading back.  Once per step,
+``kv4_append`` finds room for the new tokens.  For long contexts
+``kv4_summarize`` keeps the mean key of every page and ``kv4_select`` picks the
+pages that ``kv4_attention`` then reads.  Queries, keys and values may be slices of the fused projection;
 all calls only enqueue work on the current stream and can be captured in a HIP
 graph.  There is no backward pass and no forward-mode derivative: inputs that
 require a gradient while gradients are recorded, or that carry a tangent, are
@@ -16,7 +19,7 @@ attention to vLLM.
 from __future__ import annotations
 
 from functools import lru_cache
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -101,6 +104,28 @@ def _index(x: torch.Tensor, name: str, dtype: torch.dtype, n: int, device: torch
     return x if x.is_contiguous() else x.contiguous()
 
 
+def _table(x: torch.Tensor, seqs: int, device: torch.device) -> Tuple[torch.Tensor, int]:
+    """A page table [seqs, width] and the distance of its rows"""
+    if x.dim() != 2 or x.dtype is not torch.int32 or x.device != device or x.shape[0] != seqs:
+        raise ValueError(f"GRINQH: page_table must be torch.int32 [{seqs}, width] on {device}, got {x.dtype} "
+                         f"{list(x.shape)} on {x.device}")
+    stride, one = x.stride()
+    if one != 1:
+        x = x.contiguous()
+        stride = x.stride(0)
+    return x, stride
+
+
+def _head_table(x: torch.Tensor, seqs: int, kv_heads: int, device: torch.device) -> Tuple[torch.Tensor, int, int]:
+    """A page table [seqs, kv_heads, width] and the distances of its sequences and heads"""
+    if x.dtype is not torch.int32 or x.device != device or x.shape[:2] != (seqs, kv_heads):
+        raise ValueError(f"GRINQH: page_table must be torch.int32 [{seqs}, {kv_heads}, width] on {device}, got {x.dtype} "
+                         f"{list(x.shape)} on {x.device}")
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    return x, x.stride(0), x.stride(1)
+
+
 _stream = torch._C._cuda_getCurrentRawStream  # current_stream() without its wrapper object
 
 
@@ -157,8 +182,9 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                   scale: Optional[float] = None) -> torch.Tensor:
     """Attention of one query token per sequence, ``q [seqs, heads, head_dim]``, over the first ``lengths[s]`` (int32)
-    tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  ``scale`` defaults to head_dim ** -0.5.  A length
-    of 0 gives zeros; a length past the table or a page outside the cache NaN."""
+    tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``, or ``[seqs, kv_heads, width]``: a choice of pages
+    per key/value head, as ``kv4_select`` makes it).  ``scale`` defaults to head_dim ** -0.5.  A length of 0 gives
+    zeros; a length past the table or a page outside the cache NaN."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
     dev, dtype = cache.device, q.dtype
     dt = _dtype_code(dtype)
@@ -166,26 +192,29 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     seqs, heads, dq = q.shape
     if dq != d or heads % kv_heads:
         raise ValueError(f"GRINQH: q {tuple(q.shape)} does not match a cache of {kv_heads} heads of {d} channels")
-    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.device != dev or \
-            page_table.shape[0] != seqs:
-        raise ValueError(f"GRINQH: page_table must be torch.int32 [{seqs}, width] on {dev}, got {page_table.dtype} "
-                         f"{list(page_table.shape)} on {page_table.device}")
-    table_stride, one = page_table.stride()
-    if one != 1:
-        page_table = page_table.contiguous()
-        table_stride = page_table.stride(0)
+    if page_table.dim() == 3:
+        page_table, table_stride, table_head = _head_table(page_table, seqs, kv_heads, dev)
+    else:
+        page_table, table_stride = _table(page_table, seqs, dev)
+        table_head = None
     lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
-    width = page_table.shape[1]
+    width = page_table.shape[-1]
     out = torch.empty((seqs, heads, d), dtype=dtype, device=dev)
     with _lib.on_device(dev):
         stream = _stream(dev.index)
         nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
         ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
-        _lib.check(_lib.load_library().grinqh_kv4_attention(
-            q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
-            page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
-            "grinqh_kv4_attention")
+        lib, space = _lib.load_library(), (ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
+        if table_head is None:
+            _lib.check(lib.grinqh_kv4_attention(
+                q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
+                page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
+                *space, stream), "grinqh_kv4_attention")
+        else:
+            _lib.check(lib.grinqh_kv4_attention_selected(
+                q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
+                page_table.data_ptr(), table_stride, table_head, width, lengths.data_ptr(), _scale(scale, d),
+                out.data_ptr(), dt, *space, stream), "grinqh_kv4_attention_selected")
     return out
 
 
@@ -225,3 +254,165 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends: to
             ends.data_ptr(), key_ends.data_ptr(), seqs, tokens, keys, heads, kv_heads, d, _scale(scale, d),
             out.data_ptr(), dt, _stream(dev.index)), "grinqh_prompt_attention")
     return out
+
+
+class Appended(NamedTuple):
+    """What ``kv4_append`` found: for the rows of the batch, for its sequences and for the list of free pages."""
+    slots: torch.Tensor       # int64 [tokens], for kv4_store; -1: none
+    positions: torch.Tensor   # int32 [tokens]: place in the sequence; 0 behind the last one
+    ends: torch.Tensor        # int32 [seqs + 1]: sequence s has rows ends[s] .. ends[s + 1] - 1
+    lengths: torch.Tensor     # int32 [seqs], the new tokens counted
+    free_count: torch.Tensor  # int32 [1]
+
+
+def kv4_append(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free: torch.Tensor,
+               free_count: torch.Tensor, page_size: int, tokens: int) -> Appended:
+    """Room for ``counts[s]`` (int32 ``[seqs]``) new tokens of sequences that hold ``lengths[s]``, without the host
+    knowing either.  The pages they need beyond those they have come from the end of ``free[:free_count]`` (int32;
+    ``free_count [1]``), in the order of the sequences, and are written into ``page_table`` (int32 ``[seqs, width]``) in
+    place; nothing else that is given changes.  ``tokens`` is the number of rows of the batch's buffers, the new tokens
+    packed in front: rows behind the last sequence have slot -1, tokens that do not fit are not counted.  Where pages
+    run out the table gets -1, and where it ends nothing: such tokens have slot -1 (``kv4_store`` skips them) and the
+    attention of their sequences is NaN."""
+    dev = page_table.device
+    if not page_table.is_cuda:
+        raise ValueError(f"GRINQH: page_table must be on a HIP device (got {dev}); there is no CPU path")
+    seqs = lengths.shape[0] if lengths.dim() == 1 else -1
+    lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
+    table, table_stride = _table(page_table, seqs, dev)
+    width = table.shape[1]
+    if table is not page_table or seqs > 1 and table_stride < width:
+        raise ValueError("GRINQH: page_table is written in place: its rows must be contiguous and must not overlap, got "
+                         f"strides {page_table.stride()}")
+    table_stride = max(table_stride, width)
+    counts = _index(counts, "counts", torch.int32, seqs, dev)
+    free = _index(free, "free", torch.int32, free.numel(), dev)
+    free_count = _index(free_count, "free_count", torch.int32, 1, dev)
+    if page_size < 16 or page_size & (page_size - 1) or not 0 <= tokens < 1 << 23:
+        raise ValueError(f"GRINQH: page_size must be a power of two of at least 16, tokens from 0 to 2^23 - 1; got "
+                         f"{page_size}, {tokens}")
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    positions, ends, after, count = torch.empty(
+        tokens + 2 * seqs + 2, dtype=torch.int32, device=dev).split((tokens, seqs + 1, seqs, 1))
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().grinqh_kv4_append(
+            table.data_ptr(), table_stride, width, page_size, lengths.data_ptr(), counts.data_ptr(), seqs,
+            free.data_ptr(), free.shape[0], free_count.data_ptr(), tokens, slots.data_ptr(), positions.data_ptr(),
+            ends.data_ptr(), after.data_ptr(), count.data_ptr(), _stream(dev.index)), "grinqh_kv4_append")
+    return Appended(slots, positions, ends, after, count)
+
+
+def kv4_chunk_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                        ends: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of several new tokens per sequence, which the cache holds already: ``q [tokens, heads,
+    head_dim]``, sequence s has rows ``ends[s] .. ends[s + 1] - 1`` (int32 ``[seqs + 1]``, ascending) and the first
+    ``lengths[s]`` (int32) tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  Its last row sees all of
+    them, the row before one fewer, and so on.  Rows that see none, in front of the first sequence or behind the last
+    give zeros; a length past the table makes the sequence's rows NaN, a page outside the cache those that see it.
+    ``scale`` defaults to head_dim ** -0.5."""
+    pages, kv_heads, page, d, group = _cache_layout(cache)
+    dev, dtype = cache.device, q.dtype
+    dt = _dtype_code(dtype)
+    q, q_token, q_head = _rows(q, "q", dev, dtype)
+    tokens, heads, dq = q.shape
+    if dq != d or heads == 0 or heads % kv_heads:
+        raise ValueError(f"GRINQH: q {tuple(q.shape)} does not match a cache of {kv_heads} heads of {d} channels")
+    seqs = ends.numel() - 1
+    if seqs < 0:
+        raise ValueError(f"GRINQH: ends must be int32 [seqs + 1], got {list(ends.shape)}")
+    ends = _index(ends, "ends", torch.int32, seqs + 1, dev)
+    page_table, table_stride = _table(page_table, seqs, dev)
+    lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
+    width = page_table.shape[1]
+    lib = _lib.load_library()
+    out = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
+    nbytes = _chunk_workspace_bytes(tokens, seqs, heads, kv_heads, d, width * page)
+    # scratch of this call alone: nothing is kept in it, and a captured graph has its own
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _lib.on_device(dev):
+        _lib.check(lib.grinqh_kv4_chunk_attention(
+            q.data_ptr(), q_token, q_head, tokens, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
+            page_table.data_ptr(), table_stride, width, lengths.data_ptr(), ends.data_ptr(), seqs, _scale(scale, d),
+            out.data_ptr(), dt, ws.data_ptr() if ws is not None else None, nbytes, _stream(dev.index)),
+            "grinqh_kv4_chunk_attention")
+    return out
+
+
+@lru_cache(maxsize=1024)
+def _chunk_workspace_bytes(tokens: int, seqs: int, heads: int, kv_heads: int, head_dim: int, capacity: int) -> int:
+    return _lib.load_library().grinqh_kv4_chunk_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_dim,
+                                                                          capacity)
+
+
+def kv4_summary(cache: torch.Tensor) -> torch.Tensor:
+    """An empty summary of a cache's pages: int8 ``[pages, kv_heads, head_dim + 16]``, of every page and head the mean
+    key's codes, their step (float32 in 4 bytes) and 12 unused bytes."""
+    pages, kv_heads, _, d, _ = _cache_layout(cache)
+    return torch.zeros((pages, kv_heads, d + 16), dtype=torch.int8, device=cache.device)
+
+
+def _summary_layout(summary: torch.Tensor) -> Tuple[int, int, int]:
+    """(pages, kv_heads, head_dim) of a summary"""
+    shape = summary.shape
+    if not summary.is_cuda:
+        raise ValueError("GRINQH: the summary must be on a HIP device; there is no CPU path")
+    if len(shape) != 3 or shape[2] - 16 not in HEAD_DIMS or shape[1] == 0 or summary.dtype is not torch.int8 or \
+            not summary.is_contiguous():
+        raise ValueError("GRINQH: a summary is a contiguous int8 tensor [pages, kv_heads > 0, head_dim + 16] "
+                         f"(kv4_summary), got {summary.dtype} {tuple(shape)}")
+    return shape[0], shape[1], shape[2] - 16
+
+
+def kv4_summarize(cache: torch.Tensor, summary: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+                  lengths: torch.Tensor) -> None:
+    """Bring ``summary`` up to date for every page that tokens ``starts[s] .. lengths[s] - 1`` of a sequence lie in
+    (int32 ``[seqs]`` both: the lengths before and after ``kv4_append``; 0 and the lengths for all of their pages).
+    Called after ``kv4_store``.  Sequences that share a page must agree on how many of its tokens count."""
+    pages, kv_heads, page, d, group = _cache_layout(cache)
+    dev = cache.device
+    if _summary_layout(summary) != (pages, kv_heads, d) or summary.device != dev:
+        raise ValueError(f"GRINQH: summary {tuple(summary.shape)} on {summary.device} does not match a cache of {pages} "
+                         f"pages, {kv_heads} heads of {d} channels on {dev}")
+    seqs = lengths.shape[0] if lengths.dim() == 1 else -1
+    lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
+    starts = _index(starts, "starts", torch.int32, seqs, dev)
+    page_table, table_stride = _table(page_table, seqs, dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().grinqh_kv4_summarize(
+            cache.data_ptr(), pages, kv_heads, page, d, group, summary.data_ptr(), page_table.data_ptr(), table_stride,
+            page_table.shape[1], starts.data_ptr(), lengths.data_ptr(), seqs, _stream(dev.index)),
+            "grinqh_kv4_summarize")
+
+
+def kv4_select(q: torch.Tensor, summary: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, page_size: int,
+               count: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """For one query token per sequence, ``q [seqs, heads, head_dim]``, the ``count`` (at least 2) pages of each
+    sequence and key/value head whose mean keys promise the largest logits; the first page and the last are always
+    among them.  Returns a page table per head, int32 ``[seqs, kv_heads, count]`` in the order of the sequence (-1 behind
+    the last page), and how many tokens the selected pages hold, int32 ``[seqs]``: both as ``kv4_attention`` takes them.
+    Scores are exact, equal ones go to the page that comes first."""
+    pages, kv_heads, d = _summary_layout(summary)
+    dev, dtype = summary.device, q.dtype
+    dt = _dtype_code(dtype)
+    q, q_token, q_head = _rows(q, "q", dev, dtype)
+    seqs, heads, dq = q.shape
+    if dq != d or heads == 0 or heads % kv_heads:
+        raise ValueError(f"GRINQH: q {tuple(q.shape)} does not match a summary of {kv_heads} heads of {d} channels")
+    if page_size < 16 or page_size & (page_size - 1) or count < 2:
+        raise ValueError(f"GRINQH: page_size must be a power of two of at least 16, count at least 2; got {page_size}, "
+                         f"{count}")
+    page_table, table_stride = _table(page_table, seqs, dev)
+    lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
+    width = page_table.shape[1]
+    selected = torch.empty((seqs, kv_heads, count), dtype=torch.int32, device=dev)
+    after = torch.empty(seqs, dtype=torch.int32, device=dev)
+    lib = _lib.load_library()
+    nbytes = lib.grinqh_kv4_select_workspace_bytes(seqs, kv_heads, width, count)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _lib.on_device(dev):
+        _lib.check(lib.grinqh_kv4_select(
+            q.data_ptr(), q_token, q_head, seqs, heads, summary.data_ptr(), pages, kv_heads, page_size, d,
+            page_table.data_ptr(), table_stride, width, lengths.data_ptr(), count, selected.data_ptr(),
+            after.data_ptr(), dt, ws.data_ptr() if ws is not None else None, nbytes, _stream(dev.index)),
+            "grinqh_kv4_select")
+    return selected, after
