@@ -291,10 +291,12 @@ int grinqh_kv4_append(int32_t* page_table, int64_t table_stride, int table_width
  * first lengths[s] tokens of sequence s, the last row to all of them, the row before
  * to one fewer, and so on.  Rows that see no token, in front of the first sequence
  * or behind the last give zeros; a length past the table makes the sequence's
- * results NaN, a page outside the cache those of the rows that see its tokens.
+ * results NaN, a page outside the cache those of the rows that see its tokens (and
+ * perhaps others of the sequence).
  * Tokens that a row does not see have no effect on it.  At most 2^20 sequences;
  * the workspace (..._workspace_bytes for a capacity of table_width * page_size
- * tokens, 256-byte aligned) needs no initial value and holds nothing between calls. */
+ * tokens, 256-byte aligned) is zero-filled once before its first use, as that of
+ * grinqh_kv4_attention, with which it can be one; calls that share it must be ordered. */
 size_t grinqh_kv4_chunk_attention_workspace_bytes(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_dim,
                                                   int64_t capacity);
 int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, int64_t tokens, int heads,

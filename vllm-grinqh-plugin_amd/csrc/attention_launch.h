@@ -44,6 +44,21 @@ struct Kv4Plan {
 };
 Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity);
 
+// A packed batch of chunks, and how one of the kernels that serve it shares its part
+// out (chunk_share.h).
+struct ChunkBatch {
+  const int32_t* ends;     // [seqs + 1] row offsets
+  const int32_t* lengths;  // tokens in the cache
+  int tokens, seqs, capacity;
+  int kv_heads, per;       // query heads of a key/value head
+  int64_t least_rows, most_rows;  // (token, query head) pairs of the sequences that this kernel takes
+  bool edges;              // and the rows in front of the first and behind the last
+  int block_rows, tile;    // powers of two
+  int blocks, least, most;  // runs that tiles are shared out over, tiles of a run at least, runs of a unit at most
+  int64_t units;            // at most
+  int rows_shift, tile_shift, heads_shift, per_shift;  // log2 (of kv_heads and per: -1 if it is none)
+};
+
 struct Kv4Params {
   HeadRows q;
   uint16_t* out;  // [seqs][heads][head size]
@@ -62,6 +77,8 @@ struct Kv4Params {
   float* partial;      // [plan.grid][plan.slot]
 };
 int launch_kv4_attention(const Kv4Params& p, int dtype, hipStream_t st);
+// The same for chunks of few tokens: q and out [tokens][heads][head size], plan.most, .blocks and .least from the batch.
+int launch_kv4_attention_rows(const Kv4Params& p, const ChunkBatch& batch, int dtype, hipStream_t st);
 
 struct PromptParams {
   HeadRows q, k, v;
@@ -92,15 +109,21 @@ struct AppendParams {
 };
 int launch_kv4_append(const AppendParams& p, hipStream_t st);
 
-// How kv4_chunk_attention shares its work out (chunk.hip).
+// How kv4_chunk_attention is served: sequences with up to kChunkFew (token, query head) pairs
+// per key/value head by the single-token kernel (kv4.hip), the others by the tile
+// kernel (chunk.hip), or all by one of them (plan_chunk).
+constexpr int kChunkFew = 16;
+struct ChunkPart {
+  int64_t grid;             // blocks; 0: not used
+  int64_t units;            // blocks of rows and head, at most
+  int waves, block_rows, tile;
+  int blocks, least, most;  // as in ChunkBatch
+  int64_t slot;             // floats of a run's result
+  size_t partial;           // where the runs' results stand in the workspace, in bytes
+};
 struct ChunkPlan {
-  int waves;          // per block, 32 rows each
-  int64_t units;      // blocks of rows, at most
-  int blocks;         // runs that all tiles are shared out over where a unit may be split
-  int least, most;    // tiles of a run at least, runs of a unit at most
-  int64_t grid;
-  int64_t slot;       // floats of a run's result in the workspace
-  size_t workspace;   // bytes, 0 if no unit is split
+  ChunkPart few, tiles;
+  size_t workspace;  // bytes, 0 if no unit is split; kKv4Counters counters, then the runs' results
 };
 ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity);
 
@@ -110,15 +133,11 @@ struct ChunkParams {
   Kv4Cache cache;
   const int32_t* table;
   int64_t table_stride;
-  int table_width;
-  const int32_t* lengths;
-  const int32_t* ends;  // [seqs + 1]
-  int64_t tokens;
-  int seqs, heads;
-  int sub_shift;
+  int sub_shift, heads;
   float scale;
-  ChunkPlan plan;
-  float* partial;  // [plan.grid][plan.slot]
+  ChunkBatch batch;
+  int64_t grid, slot;
+  float* partial;  // [batch.blocks][slot]
 };
 int launch_chunk_attention(const ChunkParams& p, int dtype, hipStream_t st);
 

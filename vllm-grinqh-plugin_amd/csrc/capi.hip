@@ -912,17 +912,65 @@ int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, i
   p.sub_shift = __builtin_ctz((unsigned)p.cache.sub);
   p.table = page_table;
   p.table_stride = table_stride;
-  p.table_width = table_width;
-  p.lengths = lengths;
-  p.ends = ends;
-  p.tokens = tokens;
-  p.seqs = (int)seqs;
   p.heads = heads;
   p.scale = scale;
-  p.plan = plan_chunk(tokens, seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size);
-  p.partial = static_cast<float*>(workspace);
-  if (p.plan.workspace > 0 && (workspace == nullptr || workspace_bytes < p.plan.workspace || !aligned(workspace, 256)))
+  const ChunkPlan plan = plan_chunk(tokens, seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size);
+  if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace || !aligned(workspace, 256)))
     return GRINQH_ERR_WORKSPACE;
+  uint8_t* space = static_cast<uint8_t*>(workspace);
+  auto batch = [&](const ChunkPart& part, int64_t least_rows, int64_t most_rows, bool edges) {
+    auto log2_of = [](int v) { return (v & (v - 1)) == 0 ? __builtin_ctz((unsigned)v) : -1; };
+    ChunkBatch b;
+    b.ends = ends;
+    b.lengths = lengths;
+    b.tokens = (int)tokens;
+    b.seqs = (int)seqs;
+    b.capacity = table_width * page_size;
+    b.kv_heads = kv_heads;
+    b.per = heads / kv_heads;
+    b.least_rows = least_rows;
+    b.most_rows = most_rows;
+    b.edges = edges;
+    b.block_rows = part.block_rows;
+    b.tile = part.tile;
+    b.blocks = part.blocks;
+    b.least = part.least;
+    b.most = part.most;
+    b.units = part.units;
+    b.rows_shift = log2_of(part.block_rows);
+    b.tile_shift = log2_of(part.tile);
+    b.heads_shift = log2_of(kv_heads);
+    b.per_shift = log2_of(b.per);
+    return b;
+  };
+  const bool few = plan.few.grid > 0, tiles = plan.tiles.grid > 0;
+  if (few) {
+    Kv4Params r;
+    r.q = p.q;
+    r.out = p.out;
+    r.cache = p.cache;
+    r.table = page_table;
+    r.table_stride = table_stride;
+    r.table_head = 0;
+    r.table_width = table_width;
+    r.lengths = lengths;
+    r.seqs = (int)seqs;
+    r.heads = heads;
+    r.sub_shift = p.sub_shift;
+    r.scale = scale;
+    r.plan = Kv4Plan{plan.few.waves, plan.few.blocks,    plan.few.least, plan.few.most, (int)plan.few.slot,
+                     plan.few.grid,  plan.workspace};
+    r.units = 0;
+    r.counters = reinterpret_cast<uint32_t*>(space);
+    r.partial = reinterpret_cast<float*>(space + plan.few.partial);
+    const int s = launch_kv4_attention_rows(r, batch(plan.few, 0, tiles ? kChunkFew : INT64_MAX, !tiles), dtype,
+                                            as_stream(stream));
+    if (s != GRINQH_OK || !tiles) return s;
+  }
+  p.batch = batch(plan.tiles, few ? kChunkFew + 1 : 0, INT64_MAX, true);
+  p.grid = plan.tiles.grid;
+  p.slot = plan.tiles.slot;
+  p.partial = reinterpret_cast<float*>(space + plan.tiles.partial);
   return launch_chunk_attention(p, dtype, as_stream(stream));
 }
 

@@ -10,8 +10,8 @@
 #include <type_traits>
 
 #include "attention_launch.h"
+#include "chunk_share.h"
 #include "grinqh_common.h"
-#include "wave_scan.h"
 
 namespace grinqh {
 
@@ -23,7 +23,6 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_t;
 
 constexpr int kKeys = 64;         // tokens per tile
-constexpr int kGroup = 4;         // sequences a lane looks at in a round of the plan
 constexpr float kLow = -FLT_MAX;  // running reference before the first token (finite: -inf - -inf would be NaN)
 
 __device__ __forceinline__ f32x16_t mfma32x32x16(const u32x4_t& a, const u32x4_t& b, f32x16_t c) {
@@ -47,140 +46,35 @@ __device__ __forceinline__ uint32_t result_pair(float lo, float hi) {
   return f16_pair(lo, hi);
 }
 
-// ---------------------------------------------------------------- which rows and tiles a block takes
-
-// Sequence -1 stands for the rows in front of the first sequence, sequence `seqs` for
-// those behind the last: they see no token, and their results are zeros.
-struct Sequence {
-  int row0, rows;  // tokens of the chunk
-  int length;      // tokens in the cache that count
-  bool bad;        // more than the page table covers
-};
-__device__ __forceinline__ int row_at(const ChunkParams& p, int i) {
-  return (int)min((int64_t)max(p.ends[i], 0), p.tokens);
-}
-__device__ __forceinline__ Sequence sequence(const ChunkParams& p, int s) {
-  Sequence q;
-  q.row0 = s < 0 ? 0 : row_at(p, s);
-  q.rows = max((s >= p.seqs ? (int)p.tokens : row_at(p, s + 1)) - q.row0, 0);
-  q.length = 0;
-  q.bad = false;
-  if (s >= 0 && s < p.seqs) {
-    const int64_t capacity = (int64_t)p.table_width << (p.sub_shift + 4);
-    const int length = max(p.lengths[s], 0);
-    q.bad = length > capacity;
-    q.length = q.bad ? (int)capacity : length;
-  }
-  return q;
-}
-
-struct Share {
-  Sequence q;
-  int seq, head;    // key/value head
-  int block;        // of rows, in the sequence
-  int run, runs;
-  int64_t id;       // place in the workspace of the unit's first run; the others stand `heads` apart
-};
-
-// Runs that each unit of a sequence is split into, `chunk` tiles each.
-__device__ __forceinline__ int runs_of(const ChunkParams& p, int length, int chunk) {
-  if (p.plan.most == 1) return 1;
-  return min(max(((length + kKeys - 1) / kKeys + chunk - 1) / chunk, 1), p.plan.most);
-}
-
-// Every block plans by itself from the offsets and lengths, which only the device
-// knows: units are blocks of rows and a key/value head, all tiles are shared out over
-// plan.blocks, in runs of at least plan.least tiles, all runs of a sequence alike.
-// With `joined` blocks stand for units, not runs.  False: past the last.
-__device__ __forceinline__ bool find_share(const ChunkParams& p, int64_t id, bool joined, int lane, Share& out) {
-  const int heads = p.cache.heads, per = p.heads / heads, block_rows = 32 * p.plan.waves;
-  const int64_t at = id / heads;
-  out.head = (int)(id - at * heads);
-  auto blocks_of = [&](const Sequence& q) { return (int)(((int64_t)q.rows * per + block_rows - 1) / block_rows); };
-  int chunk = 1;
-  if (p.plan.most > 1) {
-    float tiles = 0.f;
-    for (int s0 = 0; s0 < p.seqs; s0 += 64 * kGroup)
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        const int s = s0 + 64 * i + lane;
-        if (s < p.seqs) {
-          const Sequence q = sequence(p, s);
-          tiles += (float)blocks_of(q) * (float)((q.length + kKeys - 1) / kKeys);
-        }
-      }
-    const float total =
-        __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(tiles)), 63));
-    chunk = max(p.plan.least, (int)ceilf(fminf(total * (float)heads / (float)p.plan.blocks, 0x1p26f)));
-  }
-  int64_t before = 0, runs_before = 0;
-  for (int s0 = -1; s0 <= p.seqs; s0 += 64) {
-    const int s = s0 + lane;
-    int blocks = 0, runs = 1;
-    if (s <= p.seqs) {
-      const Sequence q = sequence(p, s);
-      blocks = blocks_of(q);
-      runs = runs_of(p, q.length, chunk);
-    }
-    const int items = joined ? blocks : blocks * runs;
-    const int upto = wave_scan(items), all = wave_scan(blocks * runs);
-    const uint64_t after = __ballot(before + upto > at);
-    if (after != 0) {
-      const int owner = __builtin_ctzll(after);
-      out.seq = s0 + owner;
-      out.q = sequence(p, out.seq);
-      out.runs = __builtin_amdgcn_readlane(runs, owner);
-      const int rest = (int)(at - before) - __builtin_amdgcn_readlane(upto - items, owner);
-      const int index = joined ? rest : rest / out.runs;
-      out.run = joined ? 0 : rest - index * out.runs;
-      // those with the most tokens first
-      const int count = __builtin_amdgcn_readlane(blocks, owner);
-      out.block = count - 1 - index;
-      if (index < 0 || index >= count) return false;  // offsets that are not ascending
-      out.id = (runs_before + __builtin_amdgcn_readlane(all - blocks * runs, owner) + (int64_t)index * out.runs) * heads +
-               out.head;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
-    runs_before += __builtin_amdgcn_readlane(all, 63);
-  }
-  return false;
-}
-
 // ---------------------------------------------------------------- unpacking
 
 // 8 codes as fp16 pairs minimum + scale * code (rounded once).  A nibble under the
 // exponent of 1024 is 1024 + code, one in the upper half of a byte 1024 + 16 code.
-__device__ __forceinline__ u32x4_t unpack8(uint32_t w, f16x2_t scale, f16x2_t low) {
-  const uint32_t u = w >> 8, base = 0x64006400u;
-  const f16x2_t one = {(_Float16)-1024.f, (_Float16)-1024.f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
-                less = {(_Float16)-64.f, (_Float16)-64.f};
-  auto pair = [&](uint32_t x, bool upper) {
-    const f16x2_t c = __builtin_bit_cast(f16x2_t, x | base);
+__device__ __forceinline__ u32x4_t unpack8(uint32_t w, uint32_t pair) {
+  const f16x2_t params = __builtin_bit_cast(f16x2_t, pair);
+  const f16x2_t scale = {params[0], params[0]}, low = {params[1], params[1]};
+  const uint32_t u = w >> 8;
+  const f16x2_t one = (f16x2_t)((_Float16)-1024.f), sixteenth = (f16x2_t)((_Float16)0.0625f),
+                less = (f16x2_t)((_Float16)-64.f);
+  // (x & mask) | exponents in one operation: written out, as its two constants have to be in registers
+  auto two = [&](uint32_t x, uint32_t mask, bool upper) {
+    uint32_t bits;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(bits) : "v"(x), "s"(mask), "v"(0x64006400u));
+    const f16x2_t c = __builtin_bit_cast(f16x2_t, bits);
     const f16x2_t code = upper ? __builtin_elementwise_fma(c, sixteenth, less) : c + one;
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, scale, low));
   };
-  return u32x4_t{pair(w & 0x000F000Fu, false), pair(w & 0x00F000F0u, true), pair(u & 0x000F000Fu, false),
-                 pair(u & 0x00F000F0u, true)};
+  return u32x4_t{two(w, 0x000F000Fu, false), two(w, 0x00F000F0u, true), two(u, 0x000F000Fu, false),
+                 two(u, 0x00F000F0u, true)};
 }
-__device__ __forceinline__ u32x4_t limited8(u32x4_t x) {
-  const f16x2_t most = (f16x2_t)((_Float16)65504.f);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    x[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(
-                                            __builtin_elementwise_min(__builtin_bit_cast(f16x2_t, x[i]), most), -most));
-  return x;
-}
-__device__ __forceinline__ f16x2_t both(uint32_t half) {
-  return __builtin_bit_cast(f16x2_t, (half & 0xFFFFu) * 0x00010001u);
-}
-// a parameter that is NaN or infinite
-__device__ __forceinline__ bool broken(uint32_t pair) {
-  return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
-}
-// Codes of this group may stand for more than fp16 holds (where a scale was rounded up).
-__device__ __forceinline__ bool reaching(uint32_t pair) {
-  return fmaf(15.f, fabsf(half_lo(pair)), fabsf(half_hi(pair))) > 65504.f;
+// What the largest code of a group stands for.
+__device__ __forceinline__ float reach_of(uint32_t pair) { return fmaf(15.f, half_lo(pair), half_hi(pair)); }
+// Parameters whose codes fp16 can hold.  A scale that was rounded up makes the largest
+// code stand for up to 65536: one step down brings it to 65504 at most (and the others
+// a 2^-11 of the group's range lower at most).
+__device__ __forceinline__ uint32_t within(uint32_t pair) {
+  const float most = reach_of(pair);
+  return most > 65504.f && most <= 65568.f ? pair - 1 : pair;
 }
 
 template <int N>
@@ -201,16 +95,24 @@ __device__ __forceinline__ void load_words(uint32_t (&to)[N], const uint32_t* __
   }
 }
 
-// What a thread holds of a tile, as the cache keeps it.
+// What a thread holds of a tile's keys and of its values, as the cache keeps them.
 template <int D, int WAVES>
-struct Tile {
-  static constexpr int WORDS = D / (8 * WAVES);              // of keys, and of values
-  static constexpr int VEC = WORDS < 4 ? WORDS : 4;          // tokens of one chunk of the values
-  static constexpr int PAIRS = WORDS < D / 32 ? WORDS : D / 32;
-  uint32_t k[WORDS], kp[PAIRS];
-  uint32_t v[WORDS / VEC][VEC], vp[WORDS / VEC][VEC];
-  uint32_t own;  // the key's token: its values' parameters
-  bool lost;     // its page is outside the cache
+struct Raw {
+  static constexpr int WORDS = D / (8 * WAVES);
+  static constexpr int PAIRS = WORDS < D / 32 ? WORDS : D / 32;  // of the keys' parameters
+  static constexpr int VEC = WORDS < 4 ? WORDS : 4;              // tokens of one chunk of the values
+  static constexpr int VECS = WORDS / VEC;
+};
+template <int D, int WAVES>
+struct RawKeys {
+  uint32_t w[Raw<D, WAVES>::WORDS], pair[Raw<D, WAVES>::PAIRS];
+  uint32_t value_pair;  // the token's values' parameters
+  bool lost;            // its page is outside the cache
+};
+template <int D, int WAVES>
+struct RawValues {
+  uint32_t w[Raw<D, WAVES>::VECS][Raw<D, WAVES>::VEC], pair[Raw<D, WAVES>::VECS][Raw<D, WAVES>::VEC];
+  bool lost;
 };
 
 // ---------------------------------------------------------------- the kernel
@@ -221,99 +123,97 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   // A row of keys (values) is 16 (64) bytes longer than it need be: the 32 adjacent
   // keys' chunks of one read, and 4 adjacent values' 64 bytes, then lie in different banks.
   constexpr int KEY_ROW = 2 * D + 16, VALUE_ROW = 2 * D + 64;
-  __shared__ __align__(16) uint8_t s_k[kKeys * KEY_ROW], s_v[kKeys * VALUE_ROW];
+  __shared__ __align__(16) uint8_t s_k[2][kKeys * KEY_ROW], s_v[2][kKeys * VALUE_ROW];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, half = lane >> 5;
-  Share share;
-  if (!find_share(p, blockIdx.x, false, lane, share)) return;
-  const Sequence sq = share.q;
-  const int per = p.heads / p.cache.heads;
-  const int64_t rows = (int64_t)sq.rows * per;                      // of the sequence: (token, head)
-  const int64_t row0 = ((int64_t)share.block * WAVES + wave) * 32;  // of this wave
+  ChunkShare share;
+  if (!find_chunk(p.batch, blockIdx.x, false, lane, share)) return;
+  const ChunkSequence sq = share.q;
+  const int per = p.batch.per;
+  const int rows = sq.rows * per;                      // of the sequence: (token, head)
+  const int row0 = (share.block * WAVES + wave) * 32;  // of this wave
   const bool live = row0 < rows;
   const int shift = sq.length - sq.rows;
   // this lane's row; past the last one it stands for the last and is not stored
-  const int64_t row = min(row0 + n, rows - 1);
-  const int token = (int)(row / per), head = share.head * per + (int)(row - (int64_t)token * per);
+  const int row = min(row0 + n, rows - 1);
+  const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
   const int seen = token + shift;  // last token it sees
 
   // tiles of the block's last row, and this run's share
-  const int64_t last_row = min(((int64_t)share.block + 1) * 32 * WAVES, rows) - 1;
-  const int tiles = max((int)(last_row / per) + shift + kKeys, 0) / kKeys;
-  const int part = (tiles + share.runs - 1) / share.runs;
+  const int last_row = min((share.block + 1) * (32 * WAVES), rows) - 1;
+  const int tiles = max(quotient(last_row, per, p.batch.per_shift) + shift + kKeys, 0) / kKeys;
+  const int part = share.runs == 1 ? tiles : (tiles + share.runs - 1) / share.runs;
   const int first = min(share.run * part, tiles), last = min(first + part, tiles);
   // this wave's: up to what its last row sees; masked from where its first one ends
-  const int wave_last = live ? (int)(min(row0 + 31, rows - 1) / per) + shift : -1;
-  const int wave_seen = live ? (int)(row0 / per) + shift : 0;
-  const int my_last = min(last, max(wave_last + kKeys, 0) / kKeys);
+  const int wave_seen = __builtin_amdgcn_readfirstlane(seen), wave_last = __builtin_amdgcn_readlane(seen, 31);
+  const int my_last = live ? min(last, max(wave_last + kKeys, 0) / kKeys) : 0;
 
-  // ---- a thread's share of a tile
-  using T = Tile<D, WAVES>;
-  constexpr int KEY_LANES = WAVES;  // threads per token's keys
-  const int ktok = tid / KEY_LANES, kword = tid % KEY_LANES * T::WORDS;  // token of the tile, first word
-  const int rec_of_tile = ktok >> 4;
+  // ---- a thread's share of a tile: WORDS words of one token's keys, as many of the values
+  using R = Raw<D, WAVES>;
+  const int key = tid / WAVES, key_word = tid % WAVES * R::WORDS;
+  const int rec_of_tile = wave * 64 / (16 * WAVES), value_id = tid % (16 * WAVES);  // a wave's threads share a record
+  static_assert(WAVES >= 4, "");
   const int groups = p.cache.groups, record = kv4_record_bytes(D, groups);
   const int pair_shift = __builtin_ctz((unsigned)(D / groups)) - 5;  // words i of a group share parameters
   const int last_rec = max((sq.length - 1) >> 4, 0);
   const int32_t* table = p.table + (int64_t)share.seq * p.table_stride;
+  // tiles past the sequence's end stand for its last record: nothing uses them, and every load is in bounds
   auto page_of = [&](int tile) { return table[min(4 * tile + rec_of_tile, last_rec) >> p.sub_shift]; };
-  auto load_tile = [&](T& t, int tile, int page) {
-    t.lost = (uint32_t)page >= (uint64_t)p.cache.pages;
+  auto record_of = [&](int tile, int page, bool& lost) {
+    page = __builtin_amdgcn_readfirstlane(page);
+    lost = (uint32_t)page >= (uint64_t)p.cache.pages;
     const int rec = min(4 * tile + rec_of_tile, last_rec);
-    const uint8_t* at = p.cache.p + ((((int64_t)(t.lost ? 0 : page) * p.cache.heads + share.head) << p.sub_shift) +
-                                     (rec & (p.cache.sub - 1))) * record;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(at);
-    load_words(t.k, w + (ktok & 15) * (D / 8) + kword);
+    return reinterpret_cast<const uint32_t*>(
+        p.cache.p + ((((int64_t)(lost ? 0 : page) * p.cache.heads + share.head) << p.sub_shift) +
+                     (rec & (p.cache.sub - 1))) * record);
+  };
+  auto load_keys = [&](RawKeys<D, WAVES>& t, int tile, int page) {
+    const uint32_t* w = record_of(tile, page, t.lost);
+    load_words(t.w, w + (key & 15) * (D / 8) + key_word);
 #pragma unroll
-    for (int i = 0; i < T::PAIRS; ++i) t.kp[i] = w[2 * D + (((kword + i) % W) >> pair_shift) * 16 + (ktok & 15)];
-    const uint32_t* v = w + 2 * D + 16 * groups;
-    t.own = v[2 * D + (ktok & 15)];
-    const int x = tid % (16 * WAVES);
+    for (int i = 0; i < R::PAIRS; ++i) t.pair[i] = w[2 * D + (((key_word + i) % W) >> pair_shift) * 16 + (key & 15)];
+    t.value_pair = w[4 * D + 16 * groups + (key & 15)];
+  };
+  auto load_values = [&](RawValues<D, WAVES>& t, int tile, int page) {
+    const uint32_t* v = record_of(tile, page, t.lost) + 2 * D + 16 * groups;
 #pragma unroll
-    for (int j = 0; j < T::WORDS / T::VEC; ++j) {
-      const int id = x + 16 * WAVES * j, chunk = id % (D / 8), tok = id / (D / 8) * T::VEC;
-      load_words(t.v[j], v + chunk * 16 + tok);
-      load_words(t.vp[j], v + 2 * D + tok);
+    for (int j = 0; j < R::VECS; ++j) {
+      const int id = value_id + 16 * WAVES * j, chunk = id % (D / 8), token = id / (D / 8) * R::VEC;
+      load_words(t.w[j], v + chunk * 16 + token);
+      load_words(t.pair[j], v + 2 * D + token);
     }
   };
   // A token whose values are NaN (or lie outside the cache) gives zeros, and NaN as
-  // its key: that reaches the rows that see it and no others, as the others' logits are masked.
-  auto write_tile = [&](const T& t) {
-    bool far = false;
-    uint32_t kp[T::PAIRS];
+  // its key: that reaches the rows that see it and no others, as the others' logits are
+  // masked.  So does what no token was stored as, which stands behind a sequence's end and
+  // must only stay finite.  All that takes one test in most tiles.
+  auto settle_raw = [&](RawKeys<D, WAVES>& k, RawValues<D, WAVES>& v) {
+    float reach = fabsf(reach_of(k.value_pair));
 #pragma unroll
-    for (int i = 0; i < T::PAIRS; ++i) {
-      kp[i] = t.lost || broken(t.own) ? 0x7E007E00u : t.kp[i];
-      far |= reaching(kp[i]);
-    }
-    far = __any(far);
+    for (int i = 0; i < R::PAIRS; ++i) reach += fabsf(reach_of(k.pair[i]));
 #pragma unroll
-    for (int i = 0; i < T::WORDS; ++i) {
-      const int word = kword + i, chunk = word / W + 4 * (word % W);
-      const uint32_t pair = kp[i % T::PAIRS];
-      u32x4_t x = unpack8(t.k[i], both(pair), both(pair >> 16));
-      if (far) x = limited8(x);
-      *reinterpret_cast<u32x4_t*>(s_k + ktok * KEY_ROW + chunk * 16) = x;
-    }
-    const int x0 = tid % (16 * WAVES), base = tid / (16 * WAVES) * 16;
+    for (int j = 0; j < R::VECS; ++j)
 #pragma unroll
-    for (int j = 0; j < T::WORDS / T::VEC; ++j) {
-      const int id = x0 + 16 * WAVES * j, chunk = id % (D / 8), tok = id / (D / 8) * T::VEC;
-      uint32_t vp[T::VEC];
-      far = false;
+      for (int e = 0; e < R::VEC; ++e) reach += fabsf(reach_of(v.pair[j][e]));
+    if (!__any(!(reach <= 65504.f)) && !k.lost && !v.lost) return;
+    auto beyond = [](uint32_t pair) { return !(fabsf(reach_of(pair)) <= 65568.f); };
 #pragma unroll
-      for (int e = 0; e < T::VEC; ++e) {
-        vp[e] = t.lost || broken(t.vp[j][e]) ? 0u : t.vp[j][e];
-        far |= reaching(vp[e]);
-      }
-      far = __any(far);
+    for (int i = 0; i < R::PAIRS; ++i) k.pair[i] = k.lost || beyond(k.value_pair) ? 0x7E007E00u : within(k.pair[i]);
 #pragma unroll
-      for (int e = 0; e < T::VEC; ++e) {
-        u32x4_t x = unpack8(t.v[j][e], both(vp[e]), both(vp[e] >> 16));
-        if (far) x = limited8(x);
-        *reinterpret_cast<u32x4_t*>(s_v + (base + tok + e) * VALUE_ROW + chunk * 16) = x;
-      }
-    }
+    for (int j = 0; j < R::VECS; ++j)
+#pragma unroll
+      for (int e = 0; e < R::VEC; ++e) v.pair[j][e] = v.lost || beyond(v.pair[j][e]) ? 0u : within(v.pair[j][e]);
+  };
+  auto write_key = [&](const RawKeys<D, WAVES>& t, int i, uint8_t* to) {
+    const int word = key_word + i, chunk = word / W + 4 * (word % W);
+    const u32x4_t x = unpack8(t.w[i], t.pair[i % R::PAIRS]);
+    *reinterpret_cast<u32x4_t*>(to + key * KEY_ROW + chunk * 16) = x;
+  };
+  auto write_value = [&](const RawValues<D, WAVES>& t, int i, uint8_t* to) {
+    const int j = i / R::VEC, e = i % R::VEC;
+    const int id = value_id + 16 * WAVES * j, chunk = id % (D / 8), token = id / (D / 8) * R::VEC + e;
+    const u32x4_t x = unpack8(t.w[j][e], t.pair[j][e]);
+    *reinterpret_cast<u32x4_t*>(to + (16 * rec_of_tile + token) * VALUE_ROW + chunk * 16) = x;
   };
 
   // ---- queries: row n, channels 16 s + 8 half + e, brought to 2^13 <= max < 2^14 by a power of two
@@ -356,31 +256,45 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   // channel 32 m + n, keys 16 t + 4 half + 0..3 and + 8.
   const int key_base = n * KEY_ROW + 16 * half;
   const int value_base = (4 * half + ((lane & 15) >> 2)) * VALUE_ROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-  auto read_key = [&](int b, int s) {
-    return *reinterpret_cast<const u32x4_t*>(s_k + key_base + 32 * b * KEY_ROW + 32 * s);
+  auto read_key = [&](const uint8_t* kt, int b, int s) {
+    return *reinterpret_cast<const u32x4_t*>(kt + key_base + 32 * b * KEY_ROW + 32 * s);
   };
-  auto read_value = [&](int t, int m) {
+  auto read_value = [&](const uint8_t* vt, int t, int m) {
     u32x4_t a;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s16x4_t)(s_v + value_base + (16 * t + 8 * u) * VALUE_ROW + 64 * m));
+          (lds_s16x4_t)(vt + value_base + (16 * t + 8 * u) * VALUE_ROW + 64 * m));
       const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
       a[2 * u] = y[0];
       a[2 * u + 1] = y[1];
     }
     return a;
   };
-  auto compute = [&](int tile) {
-    f32x16_t S[2];
+  // S zs is exact in the exponent and M is not: the same factor for all tokens of a row,
+  // but of more than 2^16 for logits past 2^28.  With `far` the product is rounded first.
+  auto product_first = [&](f32x16_t (&S)[2]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        S[b][e] *= unit;
+        asm volatile("" : "+v"(S[b][e]));  // not contracted with the subtraction
+      }
+  };
+  auto largest = [&](const f32x16_t (&S)[2]) {
     float top = -__builtin_inff();
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      S[b] = (f32x16_t)(0.f);
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) S[b] = mfma32x32x16(read_key(b, s), qf[s], S[b]);
-    }
+      for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(top, S[b][e]), S[b][e + 1]);
+    return top;
+  };
+  // Makes S of a tile ready for its weights: the mask where the tile reaches past the
+  // wave's first row's last token, and the reference raised where a weight would pass 2^8.
+  auto settle = [&](f32x16_t (&S)[2], float top, int tile) {
     if (tile * kKeys + kKeys - 1 > wave_seen) {
+      asm volatile("");  // a branch: as selects, this is a fourth of every tile's instructions
       // last token of this tile that the row sees, less the half's 4 (compared with constants)
       const int upto = seen - tile * kKeys - 4 * half;
 #pragma unroll
@@ -388,36 +302,20 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (32 * b + (e & 3) + 8 * (e >> 2) > upto) S[b][e] = -__builtin_inff();
+      top = largest(S);
     }
-    // S zs is exact in the exponent and M is not: the same factor for all tokens of a
-    // row, but of more than 2^16 for logits past 2^28.  With `far` the product is rounded first.
-    auto product_first = [&]() {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          S[b][e] *= unit;
-          asm volatile("" : "+v"(S[b][e]));  // not contracted with the subtraction
-        }
-    };
-    if (far) product_first();
-    auto reach = [&]() {
-      top = -__builtin_inff();
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, S[b][e]);
-    };
-    reach();
+    if (far) {
+      product_first(S);
+      top = largest(S);
+    }
     if (__any(fmaf(top, zs, -M) > 8.f)) {
       float m = fmaxf(M, top * zs);
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       if (!far && __any(fabsf(m) > 0x1p24f && m != kLow)) {
         far = true;
         zs = 1.f;
-        product_first();
-        reach();
-        m = fmaxf(M, top);
+        product_first(S);
+        m = fmaxf(M, largest(S));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
       }
       const float f = __builtin_amdgcn_exp2f(M - m);
@@ -426,37 +324,127 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
 #pragma unroll
       for (int t = 0; t < MT; ++t) O[t] *= f;
     }
-    u32x4_t P[4];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * i], zs, -M));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * i + 1], zs, -M));
-        sum += p0 + p1;
-        P[2 * b + (i >> 2)][i & 3] = f16_pair(p0, p1);
-      }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) O[m] = mfma32x32x16(read_value(t, m), P[t], O[m]);
+  };
+  u32x4_t P[4];
+  // Weights of two tokens, pair q of key block b, as fp16 for the second product (2^-11 of
+  // them at most); they are summed as rounded, in fp32.
+  auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], zs, -M));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], zs, -M));
+    const uint32_t pair = f16_pair(p0, p1);
+    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), (f16x2_t)((_Float16)1.f), sum, false);
+    P[2 * b + (q >> 2)][q & 3] = pair;
   };
 
-  T t;
-  int page = 0;
-  if (first < last) {
-    load_tile(t, first, page_of(first));
-    page = page_of(first + 1);
-  }
-  for (int tile = first; tile < last; ++tile) {
-    __syncthreads();  // the tile before has been read
-    write_tile(t);
-    if (tile + 1 < last) {
-      load_tile(t, tile + 1, page);
-      page = page_of(tile + 2);
+  RawKeys<D, WAVES> keys;
+  RawValues<D, WAVES> values;
+  // One tile: its weights and its part of O, and the products of the next tile, slot by
+  // slot: every slot gives the matrix unit one product and the vector unit a share
+  // of the exponentials and of the unpacking (keys two tiles ahead, values one).
+  constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = 3;
+  auto step = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], const uint8_t* kt, const uint8_t* vt, uint8_t* k_to, uint8_t* v_to,
+                  float& top) {
+    u32x4_t f[AHEAD + 1];
+    auto read = [&](int at) {  // the A operand of slot `at`
+      f[at % (AHEAD + 1)] =
+          at < KSLOTS ? read_key(kt, at / STEPS, at % STEPS) : read_value(vt, (at - KSLOTS) / MT, (at - KSLOTS) % MT);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) read(k);
+    settle_raw(keys, values);
+    int done = 0, packed = 0;
+#pragma unroll
+    for (int k = 0; k < KSLOTS; ++k) {
+      const int b = k / STEPS, s = k % STEPS;
+      read(k + AHEAD);
+      N[b] = mfma32x32x16(f[k % (AHEAD + 1)], qf[s], s == 0 ? (f32x16_t)(0.f) : N[b]);
+#pragma unroll
+      for (; done < (k + 1) * 8 / KSLOTS; ++done) weigh(S, 0, done);
+#pragma unroll
+      for (; packed < (k + 1) * R::WORDS / KSLOTS; ++packed) write_key(keys, packed, k_to);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    done = packed = 0;
+    int seen_of = 0;
+    top = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < VSLOTS; ++k) {
+      const int t = k / MT, m = k % MT;
+      if (k + AHEAD < VSLOTS) read(KSLOTS + k + AHEAD);
+      O[m] = mfma32x32x16(f[(KSLOTS + k) % (AHEAD + 1)], P[t], O[m]);
+      if (k < VSLOTS / 2) {
+#pragma unroll
+        for (; done < (k + 1) * 8 / (VSLOTS / 2); ++done) weigh(S, 1, done);
+      } else {
+#pragma unroll
+        for (; seen_of < (k + 1 - VSLOTS / 2) * 16 / (VSLOTS / 2); ++seen_of)
+          top = fmaxf(fmaxf(top, N[seen_of >> 3][2 * (seen_of & 7)]), N[seen_of >> 3][2 * (seen_of & 7) + 1]);
+      }
+#pragma unroll
+      for (; packed < (k + 1) * R::WORDS / VSLOTS; ++packed) write_value(values, packed, v_to);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto feed_keys = [&](uint8_t* to) {
+#pragma unroll
+    for (int i = 0; i < R::WORDS; ++i) write_key(keys, i, to);
+  };
+  auto feed_values = [&](uint8_t* to) {
+#pragma unroll
+    for (int i = 0; i < R::WORDS; ++i) write_value(values, i, to);
+  };
+
+  // Keys run one tile ahead of the values: while tile j is weighed, S of tile j + 1 is
+  // computed, keys of j + 2 and values of j + 1 are unpacked, and those of j + 3 and j + 2
+  // are on their way.  After the wave's last tile S is computed from whatever LDS
+  // holds, and not used.
+  f32x16_t Sa[2], Sb[2];
+  float top = 0.f;
+  int page = 0, page_before = 0;  // of the keys' and the values' next loads
+  if (first < last) {
+    const int page0 = page_of(first), page1 = page_of(first + 1);
+    page_before = page_of(first + 2);
+    load_keys(keys, first, page0);
+    load_values(values, first, page0);
+    settle_raw(keys, values);
+    feed_keys(s_k[0]);
+    feed_values(s_v[0]);
+    load_keys(keys, first + 1, page1);
+    load_values(values, first + 1, page1);
+    settle_raw(keys, values);
+    feed_keys(s_k[1]);
+    load_keys(keys, first + 2, page_before);
+    page = page_of(first + 3);
     __syncthreads();
-    if (tile < my_last) compute(tile);
+    if (first < my_last) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        Sa[b] = (f32x16_t)(0.f);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) Sa[b] = mfma32x32x16(read_key(s_k[0], b, s), qf[s], Sa[b]);
+      }
+      settle(Sa, largest(Sa), first);
+    }
+  }
+  auto turn = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], int j, int at) {  // at: j - first is odd
+    __syncthreads();
+    if (j < my_last) {
+      step(S, N, s_k[at ^ 1], s_v[at], s_k[at], s_v[at ^ 1], top);
+    } else {
+      settle_raw(keys, values);
+      feed_keys(s_k[at]);
+      feed_values(s_v[at ^ 1]);
+    }
+    load_values(values, j + 2, page_before);
+    load_keys(keys, j + 3, page);
+    page_before = page;
+    page = page_of(j + 4);
+    if (j + 1 < my_last) settle(N, top, j + 1);
+  };
+  for (int j = first; j < last; j += 2) {
+    turn(Sa, Sb, j, 0);
+    if (j + 1 >= last) break;
+    turn(Sb, Sa, j + 1, 1);
   }
   if (!live) return;
 
@@ -465,7 +453,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   const bool mine = row0 + n < rows;
   if (share.runs > 1) {
     const int r = wave * 32 + n;
-    float* slot = p.partial + (share.id + (int64_t)share.run * p.cache.heads) * p.plan.slot;
+    float* slot = p.partial + (share.slot + share.run) * p.slot;
     if (mine) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -497,18 +485,17 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
   constexpr int ROWS = 1024 / D;
-  const int block_rows = 32 * p.plan.waves, parts = block_rows / ROWS;
+  const int block_rows = p.batch.block_rows, parts = block_rows / ROWS;
   const int lane = threadIdx.x & 63;
-  Share share;
-  if (!find_share(p, blockIdx.x / parts, true, lane, share) || share.runs == 1) return;
-  if (share.id + (int64_t)(share.runs - 1) * p.cache.heads >= p.plan.grid) return;  // offsets that are not ascending
-  const int per = p.heads / p.cache.heads;
+  ChunkShare share;
+  if (!find_chunk(p.batch, blockIdx.x / parts, true, lane, share)) return;
+  const int per = p.batch.per;
   const int r = (int)(blockIdx.x % parts) * ROWS + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4) * 4;
-  const int64_t row = (int64_t)share.block * block_rows + r;
-  if (row >= (int64_t)share.q.rows * per) return;
-  const int token = (int)(row / per), head = share.head * per + (int)(row - (int64_t)token * per);
-  const float* slot = p.partial + share.id * p.plan.slot;
-  const int64_t step = (int64_t)p.cache.heads * p.plan.slot;
+  const int row = share.block * block_rows + r;
+  if (row >= share.q.rows * per) return;
+  const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
+  const float* slot = p.partial + share.slot * p.slot;
+  const int64_t step = p.slot;
   float M = kLow, sum = 0.f;
   for (int i = 0; i < share.runs; ++i) M = fmaxf(M, slot[i * step + block_rows * D + r]);
   f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -528,45 +515,66 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
 
 }  // namespace
 
+// The single-token kernel unpacks a token once for 16 rows, the tile kernel for 256
+// (128), whether it has them or not. How many rows each sequence has is known on the
+// device only: a batch with up to kChunkFew on average goes to the first as a whole
+// (any number is right in either kernel), one sequence with more to the second, and
+// several with more on average to both, each kernel taking its own.
 ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity) {
-  const int per = heads / kv_heads;
-  ChunkPlan plan;
-  plan.waves = head_size > 128 ? 4 : 8;
-  if (head_size <= 128 && tokens * per <= 64 * seqs) plan.waves = 2;
-  const int64_t block_rows = 32 * plan.waves;
+  const int64_t per = heads / kv_heads, rows = tokens * per;
+  const bool few = rows <= kChunkFew * seqs, both = !few && seqs > 1 && per <= kChunkFew;
+  ChunkPlan plan = {};
+  auto fill = [&](ChunkPart& part, int64_t units, int most) {
+    const int64_t longest = ((capacity + part.tile - 1) / part.tile + part.least - 1) / part.least;
+    part.units = units;
+    part.most = (int)(longest < 1 ? 1 : longest < most ? longest : most);
+    const int64_t more = units * (part.most - 1);
+    part.grid = units + (more < part.blocks ? more : part.blocks);
+    part.slot = (int64_t)part.block_rows * (head_size + 2);
+    if (part.most == 1) return;
+    if (plan.workspace == 0) plan.workspace = kKv4Counters * sizeof(uint32_t);
+    part.partial = plan.workspace;
+    plan.workspace += ((size_t)(part.blocks * part.slot) * sizeof(float) + 255) / 256 * 256;
+  };
   // a partial block for every sequence and for the rows in front of them and behind
-  const int64_t blocks = (tokens * per + block_rows - 1) / block_rows + seqs + 2;
-  plan.units = blocks * kv_heads;
-  plan.blocks = plan.waves == 2 ? 1024 : 256;
-  plan.least = 4;
-  const int64_t tiles = (capacity + kKeys - 1) / kKeys;
-  plan.most = plan.units < plan.blocks && tiles > plan.least ? 64 : 1;
-  plan.grid = plan.units;
-  plan.slot = block_rows * (head_size + 2);
-  plan.workspace = 0;
-  if (plan.most > 1) {
-    const int64_t longest = (tiles + plan.least - 1) / plan.least;
-    plan.most = longest < plan.most ? (int)longest : plan.most;
-    // a unit has at most one run more than its share of plan.blocks
-    const int64_t more = plan.units * (plan.most - 1);
-    plan.grid += more < plan.blocks ? more : plan.blocks;
-    plan.workspace = (size_t)plan.grid * plan.slot * sizeof(float);
+  auto units_of = [&](int64_t block_rows) { return ((rows + block_rows - 1) / block_rows + seqs + 2) * kv_heads; };
+  if (few || both) {
+    const int64_t units = both ? seqs * kv_heads : units_of(kChunkFew);
+    // as many as there are if all sequences have equally many rows
+    const Kv4Plan like = plan_kv4(seqs * kv_heads * (few ? (rows / seqs + kChunkFew - 1) / kChunkFew : 1), 1, 1,
+                                  head_size, capacity);
+    plan.few.waves = like.waves;
+    plan.few.block_rows = kChunkFew;
+    plan.few.tile = 32;
+    plan.few.blocks = like.blocks;
+    // Of a few thousand tokens (8 sequences of 3000, 2 tokens each: 15.8 us with 16 steps, 18.0
+    // with 32); short ones are not split (32 of 600: 11.5, 9.9 unsplit).
+    plan.few.least = 16;
+    fill(plan.few, units, units <= kKv4Counters ? 256 : 1);
+  }
+  if (!few) {
+    plan.tiles.waves = head_size > 128 ? 4 : 8;
+    plan.tiles.block_rows = 32 * plan.tiles.waves;
+    plan.tiles.tile = kKeys;
+    plan.tiles.blocks = 256;
+    plan.tiles.least = 8;
+    const int64_t units = units_of(plan.tiles.block_rows);
+    fill(plan.tiles, units, units < 4 * plan.tiles.blocks ? 64 : 1);
   }
   return plan;
 }
 
 int launch_chunk_attention(const ChunkParams& p, int dtype, hipStream_t st) {
-  const int64_t joins = p.plan.units * 32 * p.plan.waves * p.cache.head_size / 1024;
-  if (p.plan.grid > INT32_MAX || (p.plan.most > 1 && joins > INT32_MAX)) return GRINQH_ERR_INVALID;
+  // a split unit has two runs at least
+  const int64_t units = p.batch.units < p.batch.blocks / 2 ? p.batch.units : p.batch.blocks / 2;
+  const int64_t joins = units * p.batch.block_rows * p.cache.head_size / 1024;
+  const bool split = p.batch.most > 1;
+  if (p.grid > INT32_MAX) return GRINQH_ERR_INVALID;
   auto go = [&](auto bf, auto d) -> int {
     constexpr bool BF = decltype(bf)::value;
-    constexpr int D = decltype(d)::value, WIDE = D > 128 ? 4 : 8;
-    auto kernel = chunk_attention_kernel<BF, D, WIDE>;
-    if constexpr (D <= 128)
-      if (p.plan.waves == 2) kernel = chunk_attention_kernel<BF, D, 2>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)p.plan.grid), dim3(64 * p.plan.waves), 0, st, p);
-    if (p.plan.most > 1)
-      hipLaunchKernelGGL((chunk_join_kernel<BF, D>), dim3((uint32_t)joins), dim3(256), 0, st, p);
+    constexpr int D = decltype(d)::value, WAVES = D > 128 ? 4 : 8;
+    hipLaunchKernelGGL((chunk_attention_kernel<BF, D, WAVES>), dim3((uint32_t)p.grid), dim3(64 * WAVES), 0, st, p);
+    if (split) hipLaunchKernelGGL((chunk_join_kernel<BF, D>), dim3((uint32_t)joins), dim3(256), 0, st, p);
     return hipGetLastError() == hipSuccess ? GRINQH_OK : GRINQH_ERR_HIP;
   };
   auto sized = [&](auto bf) -> int {

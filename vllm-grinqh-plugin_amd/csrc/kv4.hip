@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "attention_launch.h"
+#include "chunk_share.h"
 #include "grinqh_common.h"
 #include "splitk_complete.h"
 #include "wave_scan.h"
@@ -343,8 +344,15 @@ __device__ __forceinline__ void load_tokens(Tokens<D, G>& t, const uint8_t* __re
 // the values' size.  Queries are brought to 2^13 <= max < 2^14 by a power of two
 // (exact), so fp16 holds them for both types and the nibbles that come out
 // 16-fold can be undone on the query's side.
-template <typename DT, int D, int G, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_kernel(const Kv4Params p) {
+//
+// With a batch of chunks (B is ChunkBatch) a block's rows are up to 16 (token, query
+// head) pairs of a sequence, each of which sees one token more per token of the chunk.
+struct OneRow {  // one token per sequence
+  static constexpr int per_shift = 0;
+};
+template <typename DT, int D, int G, int WAVES, typename B>
+__global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_kernel(const Kv4Params p, const B batch) {
+  constexpr bool CHUNK = std::is_same_v<B, ChunkBatch>;
   constexpr int kWaves = WAVES, kThreads = 64 * WAVES;
   constexpr int R = kv4_record_bytes(D, G), W = D / 32, M_TILES = D < 128 ? 1 : D / 128, ACCS = D < 128 ? 4 : 8;
   __shared__ union {
@@ -359,18 +367,69 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
   __shared__ int s_last;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Share share;
-  if (!find_share(p, blockIdx.x, lane, share)) return;
-  const int seq = share.seq, first = share.first, last = share.last;
-  const int per = p.heads / p.cache.heads, tiles = p.units / p.cache.heads;
-  const int kvh = share.unit / tiles, tile = share.unit - kvh * tiles;
-  const int h0 = kvh * per + tile * kRows, rows = min(kRows, per - tile * kRows);
-  const int length = share.length;
-  bool bad = share.bad;
+  const int per = p.heads / p.cache.heads;
+  int seq, first, last, run, runs, unit, length, kvh, rows;
+  bool bad;
+  int limit, seen;        // tokens that the block's first row and the lane's row see (negative: none)
+  int row0 = 0, shift = 0;  // chunks: first of the sequence's rows, tokens in front of it
+  int64_t place = blockIdx.x;  // of this run's result in the workspace
+  int64_t q_at, out_row;  // the lane's query, the block's first result
+  if constexpr (CHUNK) {
+    ChunkShare share;
+    if (!find_chunk(batch, blockIdx.x, false, lane, share)) return;
+    const int all = share.q.rows * per;
+    row0 = share.block * kRows;
+    rows = min(kRows, all - row0);
+    seq = share.seq;
+    kvh = share.head;
+    run = share.run;
+    runs = share.runs;
+    unit = (int)share.unit;
+    place = share.slot + share.run;
+    length = share.q.length;
+    bad = share.q.bad;
+    shift = length - share.q.rows;
+    const int row = row0 + min(n, rows - 1), token = quotient(row, per, batch.per_shift);
+    limit = __builtin_amdgcn_readfirstlane(token) + shift + 1;
+    seen = token + shift + 1;
+    const int steps = max(__builtin_amdgcn_readlane(token, 15) + shift + 1 + 31, 0) >> 5;
+    const int part = runs == 1 ? steps : (steps + runs - 1) / runs;
+    first = min(run * part, steps);
+    last = min(first + part, steps);
+    q_at = (int64_t)(share.q.row0 + token) * p.q.token + (int64_t)(kvh * per + row - token * per) * p.q.head;
+    out_row = (int64_t)share.q.row0 * p.heads + kvh * per;
+  } else {
+    Share share;
+    if (!find_share(p, blockIdx.x, lane, share)) return;
+    const int tiles = p.units / p.cache.heads;
+    kvh = share.unit / tiles;
+    const int tile = share.unit - kvh * tiles, h0 = kvh * per + tile * kRows;
+    rows = min(kRows, per - tile * kRows);
+    seq = share.seq;
+    first = share.first;
+    last = share.last;
+    run = share.run;
+    runs = share.runs;
+    unit = seq * p.units + share.unit;
+    length = limit = seen = share.length;
+    bad = share.bad;
+    q_at = (int64_t)seq * p.q.token + (int64_t)(h0 + min(n, rows - 1)) * p.q.head;
+    out_row = (int64_t)seq * p.heads + h0;
+  }
+  // where a row's results go, and whether it sees any token
+  auto result_row = [&](int row) -> int64_t {
+    if constexpr (!CHUNK) return out_row + row;
+    const int token = quotient(row0 + row, per, batch.per_shift);
+    return out_row + (int64_t)token * p.heads + (row0 + row - token * per);
+  };
+  auto sees = [&](int row) {
+    if constexpr (CHUNK) return quotient(row0 + row, per, batch.per_shift) + shift >= 0;
+    return length > 0;
+  };
 
   u32x4_t qf[W];
   {
-    const uint16_t* q = p.q.p + (int64_t)seq * p.q.token + (int64_t)(h0 + min(n, rows - 1)) * p.q.head + 8 * quad;
+    const uint16_t* q = p.q.p + q_at + 8 * quad;
 #pragma unroll
     for (int s = 0; s < W; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 32 * s);
   }
@@ -490,11 +549,11 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
           z[4 * r + i] = fmaf(acc[i], half_lo(kp[i]), fmaf(half_hi(kp[i]), qsum[g], g == 0 ? 0.f : z[4 * r + i]));
       }
     }
-    if (32 * step + 32 > length) {  // tokens past the end: whatever the record holds must not count
+    if (32 * step + 32 > limit) {  // tokens past the end: whatever the record holds must not count
       asm volatile("");  // a branch: as selects, this is a sixth of every step's instructions
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (32 * step + 16 * (e >> 2) + 4 * quad + (e & 3) >= length) {
+        if (32 * step + 16 * (e >> 2) + 4 * quad + (e & 3) >= seen) {
           z[e] = -__builtin_inff();
           vp[e >> 2][e & 3] = 0;
         }
@@ -643,8 +702,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
         sh.o[wave][n][channel] = O[mt][j][i] * unit;
       }
   __syncthreads();
-  const int64_t out_row = (int64_t)seq * p.heads + h0;
-  float* slot = p.partial + (int64_t)blockIdx.x * p.plan.slot;  // [rows][D], then m and l [kRows] each
+  float* slot = p.partial + place * p.plan.slot;  // [rows][D], then m and l [kRows] each
   for (int at = threadIdx.x; at < rows * D; at += kThreads) {
     const int row = at / D, d = at % D;
     float m = s_m[0][row];
@@ -657,8 +715,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
       sum = fmaf(f, s_l[w][row], sum);
       val = fmaf(f, sh.o[w][row][d] + s_off[w][row], val);
     }
-    if (share.runs == 1) {
-      p.out[out_row * D + at] = limited<DT>(length > 0 || sum != sum ? val / sum : 0.f);
+    if (runs == 1) {
+      p.out[result_row(row) * D + d] = limited<DT>(sees(row) || sum != sum ? val / sum : 0.f);
     } else {
       store_partial(slot + at, val);
       if (d == 0) {
@@ -667,20 +725,19 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
       }
     }
   }
-  if (share.runs == 1) return;
+  if (runs == 1) return;
 
   // as in splitk_complete: the stores have completed before the count says so
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  const int unit = seq * p.units + share.unit;
-  if (threadIdx.x == 0) s_last = atomicAdd(&p.counters[unit], 1u) == (unsigned)(share.runs - 1);
+  if (threadIdx.x == 0) s_last = atomicAdd(&p.counters[unit], 1u) == (unsigned)(runs - 1);
   __syncthreads();
   if (!s_last) return;
   // Threads share out the columns (4 adjacent ones each) and, where there are
   // more threads, the runs; the first loads leave before the weights are known.
-  const int runs = share.runs, columns = rows * D / 4;
+  const int columns = rows * D / 4;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-      slot - (int64_t)share.run * p.plan.slot, (short)0, runs * p.plan.slot * 4, 0x00020000);
+      slot - (int64_t)run * p.plan.slot, (short)0, runs * p.plan.slot * 4, 0x00020000);
   constexpr int BATCH = 16;
   const int parts = max(kThreads / columns, 1), part = min((int)threadIdx.x / columns, parts);
   f32x4_t x[BATCH];
@@ -747,8 +804,9 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
       for (int i = 1; i < parts && live && part == 0; ++i) val += sh.join.sum[i * columns + column];
     }
     if (live && part == 0) {
-      const float inv = 1.f / s_l[0][row];
-      *reinterpret_cast<u32x2_t*>(p.out + out_row * D + 4 * column) =
+      const float l = s_l[0][row];
+      const float inv = !CHUNK || sees(row) || l != l ? 1.f / l : 0.f;
+      *reinterpret_cast<u32x2_t*>(p.out + result_row(row) * D + 4 * (column - row * (D / 4))) =
           u32x2_t{(uint32_t)limited<DT>(val[0] * inv) | ((uint32_t)limited<DT>(val[1] * inv) << 16),
                   (uint32_t)limited<DT>(val[2] * inv) | ((uint32_t)limited<DT>(val[3] * inv) << 16)};
     }
@@ -840,15 +898,22 @@ Kv4Plan plan_kv4(int64_t seqs, int heads, int kv_heads, int head_size, int64_t c
   return plan;
 }
 
-int launch_kv4_attention(const Kv4Params& p, int dtype, hipStream_t st) {
+template <typename B>
+int launch_attention(const Kv4Params& p, const B& batch, int dtype, hipStream_t st) {
   return dispatch_layout(dtype, p.cache.head_size, p.cache.groups, [&](auto dt, auto d, auto g) -> int {
     constexpr int D = decltype(d)::value;
     if (p.plan.grid > INT32_MAX) return GRINQH_ERR_INVALID;
-    auto kernel = p.plan.waves == 8 ? kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 8>
-                                    : kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 4>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)p.plan.grid), dim3(64 * p.plan.waves), 0, st, p);
+    auto kernel = p.plan.waves == 8 ? kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 8, B>
+                                    : kv4_attention_kernel<decltype(dt), D, decltype(g)::value, 4, B>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)p.plan.grid), dim3(64 * p.plan.waves), 0, st, p, batch);
     return status();
   });
+}
+int launch_kv4_attention(const Kv4Params& p, int dtype, hipStream_t st) {
+  return launch_attention(p, OneRow{}, dtype, st);
+}
+int launch_kv4_attention_rows(const Kv4Params& p, const ChunkBatch& batch, int dtype, hipStream_t st) {
+  return launch_attention(p, batch, dtype, st);
 }
 
 }  // namespace grinqh

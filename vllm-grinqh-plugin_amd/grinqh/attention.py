@@ -308,8 +308,8 @@ def kv4_chunk_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.
     head_dim]``, sequence s has rows ``ends[s] .. ends[s + 1] - 1`` (int32 ``[seqs + 1]``, ascending) and the first
     ``lengths[s]`` (int32) tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  Its last row sees all of
     them, the row before one fewer, and so on.  Rows that see none, in front of the first sequence or behind the last
-    give zeros; a length past the table makes the sequence's rows NaN, a page outside the cache those that see it.
-    ``scale`` defaults to head_dim ** -0.5."""
+    give zeros; a length past the table makes the sequence's rows NaN, a page outside the cache those that see it (and
+    perhaps others of the sequence).  ``scale`` defaults to head_dim ** -0.5."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
     dev, dtype = cache.device, q.dtype
     dt = _dtype_code(dtype)
@@ -324,18 +324,30 @@ def kv4_chunk_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.
     page_table, table_stride = _table(page_table, seqs, dev)
     lengths = _index(lengths, "lengths", torch.int32, seqs, dev)
     width = page_table.shape[1]
-    lib = _lib.load_library()
     out = torch.empty((tokens, heads, d), dtype=dtype, device=dev)
     nbytes = _chunk_workspace_bytes(tokens, seqs, heads, kv_heads, d, width * page)
-    # scratch of this call alone: nothing is kept in it, and a captured graph has its own
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _lib.on_device(dev):
-        _lib.check(lib.grinqh_kv4_chunk_attention(
+        stream = _stream(dev.index)
+        ws = _chunk_workspace(dev, stream, nbytes) if nbytes else None
+        _lib.check(_lib.load_library().grinqh_kv4_chunk_attention(
             q.data_ptr(), q_token, q_head, tokens, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
             page_table.data_ptr(), table_stride, width, lengths.data_ptr(), ends.data_ptr(), seqs, _scale(scale, d),
-            out.data_ptr(), dt, ws.data_ptr() if ws is not None else None, nbytes, _stream(dev.index)),
+            out.data_ptr(), dt, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
             "grinqh_kv4_chunk_attention")
     return out
+
+
+_COUNTER_BYTES = 1 << 17
+
+
+def _chunk_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """The stream's workspace; in a graph that is being captured one of its own, so that graphs replayed at the same
+    time on different streams do not meet in it (their counters are then cleared in every replay)"""
+    if not torch.cuda.is_current_stream_capturing():
+        return _WORKSPACES.get(device, stream, nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws[:_COUNTER_BYTES].zero_()
+    return ws
 
 
 @lru_cache(maxsize=1024)
