@@ -168,6 +168,7 @@ struct SelectParams {
   int32_t* selected;      // [seqs][kv_heads][count]
   int32_t* new_lengths;   // [seqs]
 };
+bool kv4_select_fits(int table_width);  // in one launch, without scores in the workspace
 int launch_kv4_select(const SelectParams& p, int dtype, hipStream_t st);
 
 }  // namespace grinqh

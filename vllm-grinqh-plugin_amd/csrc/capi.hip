@@ -998,7 +998,8 @@ int grinqh_kv4_summarize(const void* cache, int64_t pages, int kv_heads, int pag
 }
 
 size_t grinqh_kv4_select_workspace_bytes(int64_t seqs, int kv_heads, int table_width, int count) {
-  if (seqs <= 0 || seqs > kMostSeqs || kv_heads <= 0 || table_width <= count) return 0;
+  if (seqs <= 0 || seqs > kMostSeqs || kv_heads <= 0 || table_width <= count || kv4_select_fits(table_width))
+    return 0;
   return (size_t)seqs * kv_heads * table_width * sizeof(float);
 }
 

@@ -481,36 +481,38 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
                     result_pair<BF>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
 }
 
-// Joins the runs of split units: 1024 results per block, 4 per thread.
+// Joins the runs of split units, 1024 results at a time, 4 per thread.  Whether there
+// are any only the device knows, so that few blocks are launched, which take them in turn.
+constexpr int kJoinBlocks = 512;
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
   constexpr int ROWS = 1024 / D;
-  const int block_rows = p.batch.block_rows, parts = block_rows / ROWS;
-  const int lane = threadIdx.x & 63;
+  const int block_rows = p.batch.block_rows, parts = block_rows / ROWS, per = p.batch.per;
+  const int lane = threadIdx.x & 63, c = threadIdx.x % (D / 4) * 4;
   ChunkShare share;
-  if (!find_chunk(p.batch, blockIdx.x / parts, true, lane, share)) return;
-  const int per = p.batch.per;
-  const int r = (int)(blockIdx.x % parts) * ROWS + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4) * 4;
-  const int row = share.block * block_rows + r;
-  if (row >= share.q.rows * per) return;
-  const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
-  const float* slot = p.partial + share.slot * p.slot;
-  const int64_t step = p.slot;
-  float M = kLow, sum = 0.f;
-  for (int i = 0; i < share.runs; ++i) M = fmaxf(M, slot[i * step + block_rows * D + r]);
-  f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int id = blockIdx.x; find_chunk(p.batch, id / parts, true, lane, share); id += kJoinBlocks) {
+    const int r = id % parts * ROWS + threadIdx.x / (D / 4);
+    const int row = share.block * block_rows + r;
+    if (row >= share.q.rows * per) continue;
+    const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
+    const float* slot = p.partial + share.slot * p.slot;
+    const int64_t step = p.slot;
+    float M = kLow, sum = 0.f;
+    for (int i = 0; i < share.runs; ++i) M = fmaxf(M, slot[i * step + block_rows * D + r]);
+    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < share.runs; ++i) {
-    const float f = __builtin_amdgcn_exp2f(slot[i * step + block_rows * D + r] - M);
-    sum = fmaf(f, slot[i * step + block_rows * (D + 1) + r], sum);
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(slot + i * step + r * D + c);
+    for (int i = 0; i < share.runs; ++i) {
+      const float f = __builtin_amdgcn_exp2f(slot[i * step + block_rows * D + r] - M);
+      sum = fmaf(f, slot[i * step + block_rows * (D + 1) + r], sum);
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(slot + i * step + r * D + c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+    }
+    const bool sees = token + share.q.length - share.q.rows >= 0;
+    const float inv = sees || sum != sum ? 1.f / sum : 0.f;
+    *reinterpret_cast<u32x2_t*>(p.out + (((int64_t)share.q.row0 + token) * p.heads + head) * D + c) =
+        u32x2_t{result_pair<BF>(o[0] * inv, o[1] * inv), result_pair<BF>(o[2] * inv, o[3] * inv)};
   }
-  const bool sees = token + share.q.length - share.q.rows >= 0;
-  const float inv = sees || sum != sum ? 1.f / sum : 0.f;
-  *reinterpret_cast<u32x2_t*>(p.out + (((int64_t)share.q.row0 + token) * p.heads + head) * D + c) =
-      u32x2_t{result_pair<BF>(o[0] * inv, o[1] * inv), result_pair<BF>(o[2] * inv, o[3] * inv)};
 }
 
 }  // namespace
@@ -565,16 +567,13 @@ ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int 
 }
 
 int launch_chunk_attention(const ChunkParams& p, int dtype, hipStream_t st) {
-  // a split unit has two runs at least
-  const int64_t units = p.batch.units < p.batch.blocks / 2 ? p.batch.units : p.batch.blocks / 2;
-  const int64_t joins = units * p.batch.block_rows * p.cache.head_size / 1024;
   const bool split = p.batch.most > 1;
   if (p.grid > INT32_MAX) return GRINQH_ERR_INVALID;
   auto go = [&](auto bf, auto d) -> int {
     constexpr bool BF = decltype(bf)::value;
     constexpr int D = decltype(d)::value, WAVES = D > 128 ? 4 : 8;
     hipLaunchKernelGGL((chunk_attention_kernel<BF, D, WAVES>), dim3((uint32_t)p.grid), dim3(64 * WAVES), 0, st, p);
-    if (split) hipLaunchKernelGGL((chunk_join_kernel<BF, D>), dim3((uint32_t)joins), dim3(256), 0, st, p);
+    if (split) hipLaunchKernelGGL((chunk_join_kernel<BF, D>), dim3(kJoinBlocks), dim3(256), 0, st, p);
     return hipGetLastError() == hipSuccess ? GRINQH_OK : GRINQH_ERR_HIP;
   };
   auto sized = [&](auto bf) -> int {
