@@ -6,8 +6,11 @@ RMSNorm, gate_up_proj, SiLU * mul, down_proj) with random weights: the linears
 are GRINQH's, everything between qkv_proj and o_proj is ``grinqh.attention``:
 
 * ``prompt``: a packed batch of prompts, ``kv4_store`` and ``prompt_attention``;
-* ``step``: one token per sequence, ``kv4_store`` and ``kv4_attention``;
-* ``extend``: more prompt behind a cached prefix, which ``kv4_load`` brings back.
+* ``step``: one token per sequence, ``kv4_store`` and ``kv4_attention``, over all pages or over the ``select`` pages per
+  sequence and head that ``kv4_select`` picks by the summaries that ``kv4_summarize`` keeps;
+* ``extend``: several more tokens per sequence behind the cached ones, ``kv4_store`` and ``kv4_chunk_attention``.
+
+Room for the tokens is found on the GPU (``kv4_append``): no step waits for the host to know a length.
 
     python examples/decoder_attention.py          # a small model, a few steps, tokens/s
 """
@@ -52,35 +55,41 @@ class Decoder:
         self.layers = [{"qkv": Linear(hidden, width, g), "o": Linear(heads * head_dim, hidden, g),
                         "gate_up": Linear(hidden, 2 * ffn, g), "down": Linear(ffn, hidden, g),
                         "cache": ga.kv4_cache(pages, kv_heads, head_dim, page_size, key_group)} for _ in range(layers)]
+        for layer in self.layers:
+            layer["summary"] = ga.kv4_summary(layer["cache"])
         self.norm = torch.ones(hidden, dtype=torch.float16, device="cuda")
         self.freq = 10000.0 ** (-torch.arange(0, head_dim, 2, device="cuda").float() / head_dim)
-        self.free = list(range(pages))
-        self.table = torch.zeros((0, max_pages), dtype=torch.int32, device="cuda")
-        self.lengths = torch.zeros(0, dtype=torch.int32, device="cuda")
+        self.free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device="cuda")
+        self.admit(0)
 
     def admit(self, sequences: int) -> None:
-        """Room for new sequences: max_pages pages each, anywhere in the cache."""
-        rows = [[self.free.pop() for _ in range(self.max_pages)] for _ in range(sequences)]
-        self.table = torch.tensor(rows, dtype=torch.int32, device="cuda")
+        """A new batch of empty sequences; all pages are free again."""
+        self.table = torch.full((sequences, self.max_pages), -1, dtype=torch.int32, device="cuda")
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+        self.free_count = torch.full((1,), len(self.free), dtype=torch.int32, device="cuda")
 
-    def _slots(self, sequence: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
-        return self.table[sequence, position // self.page].long() * self.page + position % self.page
+    def _room(self, counts: torch.Tensor, tokens: int) -> ga.Appended:
+        """Slots, positions and row offsets of ``counts`` new tokens per sequence; ``before`` is what they had."""
+        room = ga.kv4_append(self.table, self.lengths, counts, self.free, self.free_count, self.page, tokens)
+        self.before, self.lengths, self.free_count = self.lengths, room.lengths, room.free_count
+        return room
 
     def _rotate(self, x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
         angle = position.float().view(-1, 1, 1) * self.freq
         a, b = x.float().chunk(2, -1)
         return torch.cat((a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()), -1).to(x.dtype)
 
-    def _run(self, h: torch.Tensor, position: torch.Tensor, slots: torch.Tensor, attend) -> torch.Tensor:
+    def _run(self, h: torch.Tensor, room: ga.Appended, attend) -> torch.Tensor:
+        position = room.positions
         for layer in self.layers:
             y, _, _ = rmsnorm_sigma(h, self.norm)
             q, k, v = layer["qkv"](y).split((self.heads * self.d, self.kv_heads * self.d, self.kv_heads * self.d), 1)
             q = self._rotate(q.unflatten(1, (self.heads, self.d)), position)
             k = self._rotate(k.unflatten(1, (self.kv_heads, self.d)), position)
             v = v.unflatten(1, (self.kv_heads, self.d))  # a slice of the projection, as it is
-            ga.kv4_store(layer["cache"], k, v, slots)
-            h = h + layer["o"](attend(layer["cache"], q, k, v).flatten(1))
+            ga.kv4_store(layer["cache"], k, v, room.slots)
+            ga.kv4_summarize(layer["cache"], layer["summary"], self.table, self.before, self.lengths)
+            h = h + layer["o"](attend(layer, q, k, v).flatten(1))
             y, _, _ = rmsnorm_sigma(h, self.norm)
             y, _ = silu_mul_sigma(layer["gate_up"](y))
             h = h + layer["down"](y)
@@ -88,34 +97,25 @@ class Decoder:
 
     def prompt(self, h: torch.Tensor, lens) -> torch.Tensor:
         """Hidden states of packed prompts (``lens`` tokens each); fills the cache."""
-        sequence = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens)).cuda()
-        position = torch.cat([torch.arange(n) for n in lens]).cuda()
-        ends = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
-        self.lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
-        return self._run(h, position, self._slots(sequence, position),
-                         lambda cache, q, k, v: ga.prompt_attention(q, k, v, ends))
+        room = self._room(torch.tensor(lens, dtype=torch.int32, device="cuda"), len(h))
+        return self._run(h, room, lambda layer, q, k, v: ga.prompt_attention(q, k, v, room.ends))
 
-    def step(self, h: torch.Tensor) -> torch.Tensor:
-        """One more token per sequence."""
-        position = self.lengths.long()
-        self.lengths = self.lengths + 1
-        slots = self._slots(torch.arange(len(position), device="cuda"), position)
-        return self._run(h, position, slots,
-                         lambda cache, q, k, v: ga.kv4_attention(q, cache, self.table, self.lengths))
+    def step(self, h: torch.Tensor, select: int = 0) -> torch.Tensor:
+        """One more token per sequence; with ``select`` it sees that many pages of its sequence per head."""
+        room = self._room(torch.ones_like(self.lengths), len(h))
+
+        def attend(layer, q, k, v):
+            table, lengths = self.table, self.lengths
+            if select:
+                table, lengths = ga.kv4_select(q, layer["summary"], table, lengths, self.page, select)
+            return ga.kv4_attention(q, layer["cache"], table, lengths)
+        return self._run(h, room, attend)
 
     def extend(self, h: torch.Tensor, lens) -> torch.Tensor:
         """``lens`` more tokens per sequence; their keys and values join the cached ones."""
-        before = self.lengths.tolist()
-        after = [a + b for a, b in zip(before, lens)]
-        span = lambda first, last: torch.cat([torch.arange(a, b) for a, b in zip(first, last)]).cuda()  # noqa: E731
-        owner = lambda n: torch.repeat_interleave(torch.arange(len(n)), torch.tensor(n)).cuda()  # noqa: E731
-        ends = torch.tensor([[0] + lens, [0] + after]).cumsum(1).to(torch.int32).cuda()
-        position = span(before, after)
-        every = self._slots(owner(after), span([0] * len(after), after))
-        self.lengths = torch.tensor(after, dtype=torch.int32, device="cuda")
-        return self._run(h, position, self._slots(owner(lens), position),
-                         lambda cache, q, k, v: ga.prompt_attention(q, *ga.kv4_load(cache, every, q.dtype), ends[0],
-                                                                    ends[1]))
+        room = self._room(torch.tensor(lens, dtype=torch.int32, device="cuda"), len(h))
+        return self._run(h, room, lambda layer, q, k, v: ga.kv4_chunk_attention(q, layer["cache"], self.table,
+                                                                               self.lengths, room.ends))
 
 
 def main() -> None:
@@ -127,14 +127,18 @@ def main() -> None:
     model.prompt(h, [length] * batch)
     h = torch.randn((batch, hidden), dtype=torch.float16, device="cuda")
     model.step(h)
-    torch.cuda.synchronize()
-    start = time.perf_counter()
-    for _ in range(steps):
-        h = model.step(h)
-        h = h / h.float().pow(2).mean(-1, keepdim=True).sqrt().half()
-    torch.cuda.synchronize()
-    t = (time.perf_counter() - start) / steps
-    print(f"4 layers, batch {batch}, {length} tokens of context: {t * 1e3:.2f} ms a step (eager)")
+    norm = lambda h: h / h.float().pow(2).mean(-1, keepdim=True).sqrt().half()  # noqa: E731
+    drafted = norm(model.extend(h.repeat_interleave(4, 0), [4] * batch))
+    for select in (0, 8):
+        h = drafted[3::4]
+        torch.cuda.synchronize()
+        start = time.perf_counter()
+        for _ in range(steps // 2):
+            h = norm(model.step(h, select))
+        torch.cuda.synchronize()
+        t = (time.perf_counter() - start) / (steps // 2)
+        what = f"{select} pages per head" if select else "all pages"
+        print(f"4 layers, batch {batch}, {length} tokens of context, {what}: {t * 1e3:.2f} ms a step (eager)")
 
 
 if __name__ == "__main__":
