@@ -82,6 +82,12 @@ def _chunk_case(seed, lens, news, hkv, per, d, page, group, dtype, behind=0, in_
     return cache, table, lengths, seqs, q, ends
 
 
+def _tables(table):
+    """The table, and one with room for far more: which kernel serves a sequence goes by its rows and by the table's
+    width (64 rows at most go to the single-token kernel where the table is wide, 256 where it is narrow)."""
+    return table, torch.nn.functional.pad(table, (0, 8000), value=-1)
+
+
 @pytest.mark.parametrize("dtype,d,group,page,hkv", LAYOUTS)
 @pytest.mark.parametrize("per", [1, 4, 7])
 @pytest.mark.parametrize("kind", ["few", "both", "one"])
@@ -91,13 +97,14 @@ def test_chunk(dtype, d, group, page, hkv, per, kind):
     if kind == "few":
         lens, news = [0, 1, 2, 16, 31, 33, 64, 200, 500, 7], [0, 1, 2, 1, 2, 1, 0, 2, 1, 3]
     elif kind == "both":
-        lens, news = [70, 64, 65, 127, 300, 40, 5, 0, 700, 33], [70, 1, 64, 30, 129, 1, 9, 3, 2, 0]
+        lens, news = [170, 164, 65, 227, 300, 40, 5, 0, 700, 33], [170, 1, 64, 130, 299, 1, 5, 3, 64 // per, 0]
     else:
         lens, news = [413], [150]
     case = _chunk_case(d + group + per, lens, news, hkv, per, d, page, group, dtype, behind=5, in_front=3)
     cache, table, lengths, seqs, q, ends = case
-    out = ga.kv4_chunk_attention(q, cache, table, lengths, ends)
-    _check_chunk(out, q, seqs, news, group, dtype, first=3)
+    for tab in _tables(table):
+        out = ga.kv4_chunk_attention(q, cache, tab, lengths, ends)
+        _check_chunk(out, q, seqs, news, group, dtype, first=3)
 
 
 @pytest.mark.parametrize("per", [16, 17, 40])
@@ -106,7 +113,8 @@ def test_chunk_many_query_heads(per, d):
     from grinqh import attention as ga
     for lens, news in (([70, 3, 333], [1, 3, 20]), ([200], [21])):
         cache, table, lengths, seqs, q, ends = _chunk_case(per, lens, news, 2, per, d, 32, 64, "f16")
-        _check_chunk(ga.kv4_chunk_attention(q, cache, table, lengths, ends), q, seqs, news, 64, "f16")
+        for tab in _tables(table):
+            _check_chunk(ga.kv4_chunk_attention(q, cache, tab, lengths, ends), q, seqs, news, 64, "f16")
 
 
 @pytest.mark.parametrize("lens,news", [([2777], [3]), ([2777], [40]), ([9000, 1, 513], [2, 1, 1]),
@@ -134,7 +142,8 @@ def test_chunk_many_sequences(seqs, lead):
     news[-1], lens[-1] = lead, 700
     case = _chunk_case(seqs, lens.tolist(), news.tolist(), 1, 2, 64, 16, 64, "f16", behind=100, in_front=1)
     cache, table, lengths, kv, q, ends = case
-    _check_chunk(ga.kv4_chunk_attention(q, cache, table, lengths, ends), q, kv, news.tolist(), 64, "f16", first=1)
+    for tab in (table, torch.nn.functional.pad(table, (0, 1000), value=-1)):
+        _check_chunk(ga.kv4_chunk_attention(q, cache, tab, lengths, ends), q, kv, news.tolist(), 64, "f16", first=1)
 
 
 def test_chunk_fewer_tokens_than_rows():
@@ -142,7 +151,8 @@ def test_chunk_fewer_tokens_than_rows():
     from grinqh import attention as ga
     lens, news = [40, 3, 0, 64, 5], [100, 8, 70, 64, 30]
     cache, table, lengths, seqs, q, ends = _chunk_case(4, lens, news, 2, 4, 128, 16, 32, "f16")
-    _check_chunk(ga.kv4_chunk_attention(q, cache, table, lengths, ends), q, seqs, news, 32, "f16")
+    for tab in _tables(table):
+        _check_chunk(ga.kv4_chunk_attention(q, cache, tab, lengths, ends), q, seqs, news, 32, "f16")
 
 
 @pytest.mark.parametrize("news", [[4, 2], [150, 2]])
@@ -151,6 +161,7 @@ def test_chunk_nan_reaches_only_rows_that_see_it(news, which):
     from grinqh import attention as ga
     lens = [300, 50]
     cache, table, lengths, kv, q, ends = _chunk_case(6, lens, news, 2, 4, 128, 16, 64, "f16")
+    table = _tables(table)[1]
     clean = ga.kv4_chunk_attention(q, cache, table, lengths, ends)
     row = news[0] - 2                       # the last row but one
     token = lens[0] - news[0] + row         # its own token
@@ -177,7 +188,7 @@ def test_chunk_values_at_the_limit(dtype, new):
     v[:, :, ::2] = _randn(rng, n, 1, 64, dtype=dtype) * 1000
     k[:, :, 5] = 7e4 if dtype == "bf16" else LIMIT
     cache = ga.kv4_cache(13, 1, 128, 16, 32)
-    table = _i32([[12 - i for i in range(13)]])
+    table = _tables(_i32([[12 - i for i in range(13)]]))[1]
     at = torch.arange(n).cuda()
     ga.kv4_store(cache, k, v, table[0, at // 16].long() * 16 + at % 16)
     q = _randn(rng, new, 4, 128, dtype=dtype)
@@ -196,6 +207,7 @@ def test_chunk_query_sizes_and_scale(new, size):
     from grinqh import attention as ga
     lens, news = [90, 1000], [new, new]
     cache, table, lengths, kv, q, ends = _chunk_case(5, lens, news, 2, 4, 128, 16, 32, "f16")
+    table = _tables(table)[1]
     q = q * size
     scale = 0.5 / max(1.0, size)
     _check_chunk(ga.kv4_chunk_attention(q, cache, table, lengths, ends, scale=scale), q, kv, news, 32, "f16", scale)
@@ -203,7 +215,7 @@ def test_chunk_query_sizes_and_scale(new, size):
     _check_chunk(ga.kv4_chunk_attention(qb, cache, table, lengths, ends), qb, kv, news, 32, "bf16")
 
 
-@pytest.mark.parametrize("new", [2, 40])
+@pytest.mark.parametrize("new", [2, 60])
 @pytest.mark.parametrize("size", [1e6, 1e20, 1e30])
 def test_chunk_logits_of_any_size(new, size):
     """One token's key is the query's own direction and wins by far: its value is the result, whatever the logits' size.
@@ -219,8 +231,10 @@ def test_chunk_logits_of_any_size(new, size):
     ga.kv4_store(cache, k, v, slots)
     _, kept = ga.kv4_load(cache, slots, torch.bfloat16)
     q = torch.full((new, 2, 64), size, dtype=torch.bfloat16, device="cuda")
-    out = ga.kv4_chunk_attention(q, cache, _i32([list(range(9))]), _i32([n]), _i32([0, new]))
-    want = (kept[7].float() + kept[71].float()) / 2
+    out = ga.kv4_chunk_attention(q, cache, _tables(_i32([list(range(9))]))[1], _i32([n]), _i32([0, new]))
+    # a row that ends in front of the second one (the first of 60: it sees 70 + 1 tokens) has the first one's value
+    both = (torch.arange(n - new, n) >= 71).cuda().view(-1, 1, 1)
+    want = torch.where(both, (kept[7].float() + kept[71].float()) / 2, kept[7].float())
     err = (out.float() - want).abs()
     # bf16 roundings of the two values and of the result, fp16's of the weights and values
     assert bool((err <= 2.0 ** -8 * (kept[7].float().abs() + kept[71].float().abs()) + 2.0 ** -8 * want.abs()).all())
@@ -232,6 +246,8 @@ def test_chunk_bad_pages_and_lengths():
     for news in ([3, 2, 1], [60, 70, 2]):
         lens = [200, 150, 40]
         cache, table, lengths, kv, q, ends = _chunk_case(3, lens, news, 2, 4, 128, 16, 128, "f16")
+        if news[0] > 16:
+            table = _tables(table)[1]
         clean = ga.kv4_chunk_attention(q, cache, table, lengths, ends)
         for page in (-1, cache.shape[0], 2 ** 31 - 1):
             bad = table.clone()
@@ -253,6 +269,7 @@ def test_chunk_offsets_that_are_not_ascending_stay_in_bounds():
     from grinqh import attention as ga
     lens, news = [3000, 3000, 3000], [40, 2, 70]
     cache, table, lengths, kv, q, ends = _chunk_case(2, lens, news, 2, 4, 64, 16, 64, "f16")
+    table = _tables(table)[1]
     for e in ([0, 112, 3, 112], [112, 0, 112, 0], [-5, 200, 1 << 30, -(1 << 31)], [50, 50, 2, 1]):
         ga.kv4_chunk_attention(q, cache, table, lengths, _i32(e))
     for few in (q[:7], q):
@@ -266,6 +283,7 @@ def test_chunk_strides_and_streams():
     from grinqh import attention as ga
     lens, news = [300, 50, 90], [40, 1, 7]
     cache, table, lengths, kv, q, ends = _chunk_case(12, lens, news, 2, 4, 128, 16, 32, "f16")
+    table = _tables(table)[1]
     want = ga.kv4_chunk_attention(q, cache, table, lengths, ends)
     wide = torch.randn((48, 12 * 128 + 8), device="cuda").half()
     wide[:, 8:8 + 1024] = q.flatten(1)

@@ -109,10 +109,9 @@ struct AppendParams {
 };
 int launch_kv4_append(const AppendParams& p, hipStream_t st);
 
-// How kv4_chunk_attention is served: sequences with up to kChunkFew (token, query head) pairs
+// How kv4_chunk_attention is served: sequences with up to few_rows (token, query head) pairs
 // per key/value head by the single-token kernel (kv4.hip), the others by the tile
 // kernel (chunk.hip), or all by one of them (plan_chunk).
-constexpr int kChunkFew = 16;
 struct ChunkPart {
   int64_t grid;             // blocks; 0: not used
   int64_t units;            // blocks of rows and head, at most
@@ -123,6 +122,7 @@ struct ChunkPart {
 };
 struct ChunkPlan {
   ChunkPart few, tiles;
+  int few_rows;
   size_t workspace;  // bytes, 0 if no unit is split; kKv4Counters counters, then the runs' results
 };
 ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity);

@@ -963,11 +963,11 @@ int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, i
     r.units = 0;
     r.counters = reinterpret_cast<uint32_t*>(space);
     r.partial = reinterpret_cast<float*>(space + plan.few.partial);
-    const int s = launch_kv4_attention_rows(r, batch(plan.few, 0, tiles ? kChunkFew : INT64_MAX, !tiles), dtype,
+    const int s = launch_kv4_attention_rows(r, batch(plan.few, 0, tiles ? plan.few_rows : INT64_MAX, !tiles), dtype,
                                             as_stream(stream));
     if (s != GRINQH_OK || !tiles) return s;
   }
-  p.batch = batch(plan.tiles, few ? kChunkFew + 1 : 0, INT64_MAX, true);
+  p.batch = batch(plan.tiles, few ? plan.few_rows + 1 : 0, INT64_MAX, true);
   p.grid = plan.tiles.grid;
   p.slot = plan.tiles.slot;
   p.partial = reinterpret_cast<float*>(space + plan.tiles.partial);

@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
 
 // Joins the runs of split units, 1024 results at a time, 4 per thread.  Whether there
 // are any only the device knows, so that few blocks are launched, which take them in turn.
-constexpr int kJoinBlocks = 512;
+constexpr int kJoinBlocks = 2048;
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
   constexpr int ROWS = 1024 / D;
@@ -518,14 +518,20 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
 }  // namespace
 
 // The single-token kernel unpacks a token once for 16 rows, the tile kernel for 256
-// (128), whether it has them or not. How many rows each sequence has is known on the
-// device only: a batch with up to kChunkFew on average goes to the first as a whole
-// (any number is right in either kernel), one sequence with more to the second, and
-// several with more on average to both, each kernel taking its own.
+// (128), whether it has them or not, and takes longer to start.  Which is the faster by
+// the rows of a sequence and the tiles that all have (32 query and 8 key/value heads, us;
+// 16 seqs of 2000, 32 rows: 17, 46; 1 of 32768, 64: 34, 53; 32 of 2000, 64: 44, 61,
+// 128: 78, 66; 8 of 2000, 128: 27, 40; 1 of 2000, 256: 17, 34; 32 of 2000, 256: 150, 98).
+// How many rows each sequence has is known on the device only: a batch with few on
+// average goes to the first as a whole (any number is right in either kernel), one
+// sequence with more to the second, and several with more on average to both, each
+// kernel taking its own.
 ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int head_size, int64_t capacity) {
-  const int64_t per = heads / kv_heads, rows = tokens * per;
-  const bool few = rows <= kChunkFew * seqs, both = !few && seqs > 1 && per <= kChunkFew;
+  constexpr int kRows = 16;  // of the single-token kernel's blocks
+  const int64_t per = heads / kv_heads, rows = tokens * per, all = seqs * kv_heads * ((capacity + kKeys - 1) / kKeys);
   ChunkPlan plan = {};
+  plan.few_rows = all <= 512 ? 256 : all <= 2048 ? 128 : 64;
+  const bool few = rows <= plan.few_rows * seqs, both = !few && seqs > 1 && per <= plan.few_rows;
   auto fill = [&](ChunkPart& part, int64_t units, int most) {
     const int64_t longest = ((capacity + part.tile - 1) / part.tile + part.least - 1) / part.least;
     part.units = units;
@@ -541,12 +547,12 @@ ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int 
   // a partial block for every sequence and for the rows in front of them and behind
   auto units_of = [&](int64_t block_rows) { return ((rows + block_rows - 1) / block_rows + seqs + 2) * kv_heads; };
   if (few || both) {
-    const int64_t units = both ? seqs * kv_heads : units_of(kChunkFew);
+    const int64_t units = both ? seqs * kv_heads * (plan.few_rows / kRows) : units_of(kRows);
     // as many as there are if all sequences have equally many rows
-    const Kv4Plan like = plan_kv4(seqs * kv_heads * (few ? (rows / seqs + kChunkFew - 1) / kChunkFew : 1), 1, 1,
-                                  head_size, capacity);
+    const Kv4Plan like = plan_kv4(seqs * kv_heads * (few ? (rows / seqs + kRows - 1) / kRows : 1), 1, 1, head_size,
+                                  capacity);
     plan.few.waves = like.waves;
-    plan.few.block_rows = kChunkFew;
+    plan.few.block_rows = kRows;
     plan.few.tile = 32;
     plan.few.blocks = like.blocks;
     // Of a few thousand tokens (8 sequences of 3000, 2 tokens each: 15.8 us with 16 steps, 18.0

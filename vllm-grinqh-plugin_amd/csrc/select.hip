@@ -459,13 +459,13 @@ __device__ __forceinline__ void select_top(TopShared<THREADS>& sh, int count, in
     }
   }
   if (many) {
-    low = FLT_MAX, high = -FLT_MAX;
+    float least = FLT_MAX, most = -FLT_MAX;  // not low and high, which the parts are reckoned from
     each([&](int j) {
       if (part(j) != at) return;
-      low = fminf(low, score_at(j));
-      high = fmaxf(high, score_at(j));
+      least = fminf(least, score_at(j));
+      most = fmaxf(most, score_at(j));
     });
-    range(low, high, 1, lo, hi);
+    range(least, most, 1, lo, hi);
     while (lo < hi) {
       const int shift = max(32 - __builtin_clz(hi - lo) - 11, 0);
       each([&](int j) {
