@@ -259,7 +259,9 @@ def test_chunk_bad_pages_and_lengths():
         long = lengths.clone()
         long[0] = table.shape[1] * 16 + 1
         out = ga.kv4_chunk_attention(q, cache, table.clamp_min(0), long, ends)
-        assert bool(out[:news[0]].isnan().all()) and torch.equal(out[news[0]:], clean[news[0]:])
+        assert bool(out[:news[0]].isnan().all())
+        # the other sequences' work is shared out differently beside a long one: the same within the bounds
+        _check_chunk(out[news[0]:], q[news[0]:], kv[1:], news[1:], 128, "f16")
         none = ga.kv4_chunk_attention(q, cache[:0], table, lengths, ends)
         assert bool(none.isnan().all())
 

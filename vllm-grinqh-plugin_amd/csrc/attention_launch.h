@@ -53,10 +53,12 @@ struct ChunkBatch {
   int kv_heads, per;       // query heads of a key/value head
   int64_t least_rows, most_rows;  // (token, query head) pairs of the sequences that this kernel takes
   bool edges;              // and the rows in front of the first and behind the last
-  int block_rows, tile;    // powers of two
-  int blocks, least, most;  // runs that tiles are shared out over, tiles of a run at least, runs of a unit at most
+  int block_rows, tile;    // powers of two, as `blocks`
+  // tiles are shared out over so many blocks, runs of at least so many tiles, a unit split into so many at most
+  int blocks, least, most;
   int64_t units;            // at most
-  int rows_shift, tile_shift, heads_shift, per_shift;  // log2 (of kv_heads and per: -1 if it is none)
+  int pieces;               // results that the workspace holds, where the tile kernel's blocks take equal pieces; or 0
+  int rows_shift, tile_shift, blocks_shift, heads_shift, per_shift;  // log2 (of kv_heads and per: -1 if it is none)
 };
 
 struct Kv4Params {
@@ -117,7 +119,8 @@ struct ChunkPart {
   int64_t units;            // blocks of rows and head, at most
   int waves, block_rows, tile;
   int blocks, least, most;  // as in ChunkBatch
-  int64_t slot;             // floats of a run's result
+  int64_t slot;             // floats of a run's (piece's) result
+  int pieces;               // results in the workspace
   size_t partial;           // where the runs' results stand in the workspace, in bytes
 };
 struct ChunkPlan {
@@ -137,7 +140,7 @@ struct ChunkParams {
   float scale;
   ChunkBatch batch;
   int64_t grid, slot;
-  float* partial;  // [batch.blocks][slot]
+  float* partial;  // [batch.pieces][slot]
 };
 int launch_chunk_attention(const ChunkParams& p, int dtype, hipStream_t st);
 

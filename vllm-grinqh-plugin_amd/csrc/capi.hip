@@ -937,8 +937,10 @@ int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, i
     b.least = part.least;
     b.most = part.most;
     b.units = part.units;
+    b.pieces = part.pieces;
     b.rows_shift = log2_of(part.block_rows);
     b.tile_shift = log2_of(part.tile);
+    b.blocks_shift = log2_of(part.blocks);
     b.heads_shift = log2_of(kv_heads);
     b.per_shift = log2_of(b.per);
     return b;

@@ -46,6 +46,107 @@ __device__ __forceinline__ uint32_t result_pair(float lo, float hi) {
   return f16_pair(lo, hi);
 }
 
+// ---------------------------------------------------------------- which rows and tiles a block takes
+
+// Units are blocks of rows of a sequence and a key/value head, and one block of threads fills a
+// CU.  Where there is little to do a unit is split into equal runs if there are few
+// (find_chunk).  That leaves half of the card idle with 128 long units, and 320 take as
+// long as 512.  So long ones stand on a line, each as long as its tiles take, and all blocks
+// take equal pieces of it: the end of one unit, whole ones, the beginning of another (2
+// sequences of 8000 tokens, 512 rows each, 8 heads: 270 us split into runs, 200 so; 5 of
+// 4000: 306, 248).  A unit that is cut leaves its parts in the workspace, two per block at
+// most, and a second kernel joins them, which costs as much as some 22 tiles: blocks
+// take a unit each where that is cheaper.  Lengths are in sixteenths of a tile; the d-th
+// last block of rows of a sequence is c0 + (B - d) c1 long, so that sums have a closed form
+// and every block finds its place by itself from the offsets and lengths, which only the
+// device knows.
+constexpr int kStart = 4;    // tiles that a unit takes beside its own
+constexpr int kJoining = 22;  // tiles that cutting takes
+struct Line {
+  int total, width;
+  bool pieces;  // otherwise a unit is 1 long, and its block's
+};
+struct Weight {
+  int blocks, c0, c1;
+  __device__ int before(int d) const { return d * c0 + c1 * (blocks * d - d * (d - 1) / 2); }  // blocks 0 .. d - 1
+  __device__ int of(int d) const { return c0 + (blocks - d) * c1; }
+};
+__device__ __forceinline__ Weight weight_of(const ChunkBatch& b, const ChunkSequence& q, int s, bool pieces) {
+  Weight w = {s <= b.seqs ? chunk_blocks(b, q, s) : 0, 1, 0};
+  if (pieces) {
+    w.c0 = 16 * kStart + max(q.length - q.rows, 0) / 4;
+    w.c1 = s >= 0 && s < b.seqs ? (b.block_rows + 4 * b.per - 1) / (4 * b.per) : 0;
+  }
+  return w;
+}
+// `mine`: sequence lane - 1.
+__device__ __forceinline__ Line line_of(const ChunkBatch& b, const ChunkSequence& mine, int lane) {
+  int count = 0, all = 0, longest = 0;
+  auto add = [&](const ChunkSequence& q, int s) {
+    const Weight w = weight_of(b, q, s, true);
+    count += w.blocks * b.kv_heads;
+    all += w.before(w.blocks) * b.kv_heads;
+    longest = w.blocks > 0 ? max(longest, chunk_tiles(b, q)) : longest;
+  };
+  if (lane - 1 <= b.seqs) add(mine, lane - 1);
+  for (int s = lane + 63; s <= b.seqs; s += 64) add(chunk_sequence(b, s), s);
+  count = wave_sum(count);
+  all = wave_sum(all);
+  longest = wave_reduce(longest, [](int x, int y) { return max(x, y); });
+  const int piece = (all + b.blocks - 1) >> b.blocks_shift, rounds = (count + b.blocks - 1) >> b.blocks_shift;
+  const float by_units = fmaxf((float)(longest + kStart), (float)rounds * ((float)all / (float)count) * (1.f / 16.f));
+  if (count > 0 && all > 0 && (float)piece * (1.f / 16.f) + kJoining < by_units) return {all, piece, true};
+  return {count, 1, false};
+}
+
+struct Piece {
+  ChunkSequence q;
+  int seq, head, block;  // of rows, in the sequence
+  int length, at;        // the unit's length, and where in it the place is
+};
+// What stands at place x of the line.  False: past its end.
+__device__ __forceinline__ bool find_piece(const ChunkBatch& b, const Line& l, const ChunkSequence& mine, int x, int lane,
+                                           Piece& out) {
+  int before = 0;
+  for (int s0 = -1; s0 <= b.seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const ChunkSequence q = s0 < 0 ? mine : chunk_sequence(b, s);
+    const Weight w = weight_of(b, q, s, l.pieces);
+    const int all = w.before(w.blocks) * b.kv_heads, upto = wave_scan(all);
+    const uint64_t after = __ballot(before + upto > x);
+    if (after != 0) {
+      const int owner = __builtin_ctzll(after);
+      auto of_owner = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+      const Weight o = {of_owner(w.blocks), of_owner(w.c0), of_owner(w.c1)};
+      out.seq = s0 + owner;
+      out.q = {of_owner(q.row0), of_owner(q.rows), of_owner(q.length), of_owner((int)q.bad) != 0};
+      const int rest = x - before - (of_owner(upto) - of_owner(all));
+      int d = 0, end = o.blocks;  // before(d) kv_heads <= rest < before(end) kv_heads
+      if (rest < 0 || end <= 0) return false;  // offsets that are not ascending
+      while (end - d > 1) {
+        const int mid = (d + end) >> 1;
+        if (o.before(mid) * b.kv_heads <= rest)
+          d = mid;
+        else
+          end = mid;
+      }
+      out.length = o.of(d);
+      const int inside = rest - o.before(d) * b.kv_heads;
+      if (out.length <= 0 || inside < 0) return false;
+      out.head = __builtin_amdgcn_readfirstlane(inside / out.length);  // a division leaves the scalar registers
+      out.at = inside - out.head * out.length;
+      out.block = o.blocks - 1 - d;  // those with the most tokens first
+      return out.head < b.kv_heads;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+// The tile at which a place in a unit of `tiles` tiles begins.
+__device__ __forceinline__ int tile_at(int at, int length, int tiles) {
+  return at >= length ? tiles : (int)((float)at * ((float)tiles / (float)length));
+}
+
 // ---------------------------------------------------------------- unpacking
 
 // 8 codes as fp16 pairs minimum + scale * code (rounded once).  A nibble under the
@@ -117,33 +218,82 @@ struct RawValues {
 
 // ---------------------------------------------------------------- the kernel
 
-template <bool BF, int D, int WAVES>
+// PIECES: blocks take equal pieces of all work, not a run of a unit.
+template <bool BF, int D, int WAVES, bool PIECES>
 __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_kernel(const ChunkParams p) {
   constexpr int STEPS = D / 16, MT = D / 32, W = D / 32, THREADS = 64 * WAVES;
   // A row of keys (values) is 16 (64) bytes longer than it need be: the 32 adjacent
   // keys' chunks of one read, and 4 adjacent values' 64 bytes, then lie in different banks.
   constexpr int KEY_ROW = 2 * D + 16, VALUE_ROW = 2 * D + 64;
   __shared__ __align__(16) uint8_t s_k[2][kKeys * KEY_ROW], s_v[2][kKeys * VALUE_ROW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 31, half = lane >> 5;
-  ChunkShare share;
-  if (!find_chunk(p.batch, blockIdx.x, false, lane, share)) return;
-  const ChunkSequence sq = share.q;
   const int per = p.batch.per;
+  ChunkSequence mine_of_lane;
+  Line line;
+  int begin = 0, end = 1;
+  if constexpr (PIECES) {
+    const int lane = threadIdx.x & 63;
+    mine_of_lane = chunk_sequence(p.batch, lane - 1);
+    line = line_of(p.batch, mine_of_lane, lane);
+    if ((int64_t)blockIdx.x * line.width >= line.total) return;
+    begin = (int)blockIdx.x * line.width;
+    end = min(begin + line.width, line.total);
+  }
+  for (int x = begin; x < end;) {
+  int tid = threadIdx.x;
+  if constexpr (PIECES && D <= 128) asm volatile("" : "+v"(tid));  // what follows from it is not kept between units
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
+  ChunkSequence sq;
+  int seq, kvh, block, part, place, run = 0, runs = 1, unit_length = 1, unit_at = 0;
+  bool whole;
+  if constexpr (PIECES) {
+    Piece share;
+    if (!find_piece(p.batch, line, mine_of_lane, x, lane, share)) return;
+    sq = share.q;
+    seq = share.seq;
+    kvh = share.head;
+    block = share.block;
+    unit_length = share.length;
+    unit_at = share.at;
+    part = min(unit_length - unit_at, end - x);
+    whole = part == unit_length;
+    place = 2 * (int)blockIdx.x + (x == begin ? 0 : 1);
+    if (!whole && place >= p.batch.pieces) return;  // offsets that are not ascending
+  } else {
+    ChunkShare share;
+    if (!find_chunk(p.batch, blockIdx.x, false, lane, share)) return;
+    sq = share.q;
+    seq = share.seq;
+    kvh = share.head;
+    block = share.block;
+    run = share.run;
+    runs = share.runs;
+    part = 1;
+    whole = runs == 1;
+    place = (int)share.slot + run;
+  }
   const int rows = sq.rows * per;                      // of the sequence: (token, head)
-  const int row0 = (share.block * WAVES + wave) * 32;  // of this wave
+  const int row0 = (block * WAVES + wave) * 32;  // of this wave
   const bool live = row0 < rows;
   const int shift = sq.length - sq.rows;
   // this lane's row; past the last one it stands for the last and is not stored
   const int row = min(row0 + n, rows - 1);
-  const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
+  const int token = quotient(row, per, p.batch.per_shift), head = kvh * per + row - token * per;
   const int seen = token + shift;  // last token it sees
 
   // tiles of the block's last row, and this run's share
-  const int last_row = min((share.block + 1) * (32 * WAVES), rows) - 1;
+  const int last_row = min((block + 1) * (32 * WAVES), rows) - 1;
   const int tiles = max(quotient(last_row, per, p.batch.per_shift) + shift + kKeys, 0) / kKeys;
-  const int part = share.runs == 1 ? tiles : (tiles + share.runs - 1) / share.runs;
-  const int first = min(share.run * part, tiles), last = min(first + part, tiles);
+  int first = 0, last = tiles;
+  if (!whole) {
+    if constexpr (PIECES) {
+      first = tile_at(unit_at, unit_length, tiles);
+      last = tile_at(unit_at + part, unit_length, tiles);
+    } else {
+      const int each = (tiles + runs - 1) / runs;
+      first = min(run * each, tiles);
+      last = min(first + each, tiles);
+    }
+  }
   // this wave's: up to what its last row sees; masked from where its first one ends
   const int wave_seen = __builtin_amdgcn_readfirstlane(seen), wave_last = __builtin_amdgcn_readlane(seen, 31);
   const int my_last = live ? min(last, max(wave_last + kKeys, 0) / kKeys) : 0;
@@ -156,7 +306,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   const int groups = p.cache.groups, record = kv4_record_bytes(D, groups);
   const int pair_shift = __builtin_ctz((unsigned)(D / groups)) - 5;  // words i of a group share parameters
   const int last_rec = max((sq.length - 1) >> 4, 0);
-  const int32_t* table = p.table + (int64_t)share.seq * p.table_stride;
+  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
   // tiles past the sequence's end stand for its last record: nothing uses them, and every load is in bounds
   auto page_of = [&](int tile) { return table[min(4 * tile + rec_of_tile, last_rec) >> p.sub_shift]; };
   auto record_of = [&](int tile, int page, bool& lost) {
@@ -164,7 +314,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
     lost = (uint32_t)page >= (uint64_t)p.cache.pages;
     const int rec = min(4 * tile + rec_of_tile, last_rec);
     return reinterpret_cast<const uint32_t*>(
-        p.cache.p + ((((int64_t)(lost ? 0 : page) * p.cache.heads + share.head) << p.sub_shift) +
+        p.cache.p + ((((int64_t)(lost ? 0 : page) * p.cache.heads + kvh) << p.sub_shift) +
                      (rec & (p.cache.sub - 1))) * record);
   };
   auto load_keys = [&](RawKeys<D, WAVES>& t, int tile, int page) {
@@ -187,6 +337,11 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   // its key: that reaches the rows that see it and no others, as the others' logits are
   // masked.  So does what no token was stored as, which stands behind a sequence's end and
   // must only stay finite.  All that takes one test in most tiles.
+  auto beyond = [](uint32_t pair) { return !(fabsf(reach_of(pair)) <= 65568.f); };
+  auto settle_keys = [&](RawKeys<D, WAVES>& k) {
+#pragma unroll
+    for (int i = 0; i < R::PAIRS; ++i) k.pair[i] = k.lost || beyond(k.value_pair) ? 0x7E007E00u : within(k.pair[i]);
+  };
   auto settle_raw = [&](RawKeys<D, WAVES>& k, RawValues<D, WAVES>& v) {
     float reach = fabsf(reach_of(k.value_pair));
 #pragma unroll
@@ -196,9 +351,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
 #pragma unroll
       for (int e = 0; e < R::VEC; ++e) reach += fabsf(reach_of(v.pair[j][e]));
     if (!__any(!(reach <= 65504.f)) && !k.lost && !v.lost) return;
-    auto beyond = [](uint32_t pair) { return !(fabsf(reach_of(pair)) <= 65568.f); };
-#pragma unroll
-    for (int i = 0; i < R::PAIRS; ++i) k.pair[i] = k.lost || beyond(k.value_pair) ? 0x7E007E00u : within(k.pair[i]);
+    settle_keys(k);
 #pragma unroll
     for (int j = 0; j < R::VECS; ++j)
 #pragma unroll
@@ -385,10 +538,11 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto feed_keys = [&](uint8_t* to) {
+  auto for_keys = [&](const RawKeys<D, WAVES>& t, uint8_t* to) {
 #pragma unroll
-    for (int i = 0; i < R::WORDS; ++i) write_key(keys, i, to);
+    for (int i = 0; i < R::WORDS; ++i) write_key(t, i, to);
   };
+  auto feed_keys = [&](uint8_t* to) { for_keys(keys, to); };
   auto feed_values = [&](uint8_t* to) {
 #pragma unroll
     for (int i = 0; i < R::WORDS; ++i) write_value(values, i, to);
@@ -404,17 +558,18 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   if (first < last) {
     const int page0 = page_of(first), page1 = page_of(first + 1);
     page_before = page_of(first + 2);
+    page = page_of(first + 3);
+    RawKeys<D, WAVES> second;
     load_keys(keys, first, page0);
     load_values(values, first, page0);
+    load_keys(second, first + 1, page1);
     settle_raw(keys, values);
     feed_keys(s_k[0]);
     feed_values(s_v[0]);
-    load_keys(keys, first + 1, page1);
     load_values(values, first + 1, page1);
-    settle_raw(keys, values);
-    feed_keys(s_k[1]);
     load_keys(keys, first + 2, page_before);
-    page = page_of(first + 3);
+    settle_keys(second);
+    for_keys(second, s_k[1]);
     __syncthreads();
     if (first < my_last) {
 #pragma unroll
@@ -446,71 +601,112 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
     if (j + 1 >= last) break;
     turn(Sb, Sa, j + 1, 1);
   }
-  if (!live) return;
-
-  sum += __shfl_xor(sum, 32, 64);
-  if (sq.bad) sum = __builtin_nanf("");
-  const bool mine = row0 + n < rows;
-  if (share.runs > 1) {
-    const int r = wave * 32 + n;
-    float* slot = p.partial + (share.slot + share.run) * p.slot;
-    if (mine) {
+  if (live) {
+    sum += __shfl_xor(sum, 32, 64);
+    if (sq.bad) sum = __builtin_nanf("");
+    const bool mine = row0 + n < rows;
+    if (!whole) {
+      const int r = wave * 32 + n;
+      float* slot = p.partial + (int64_t)place * p.slot;
+      if (mine) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<f32x4_t*>(slot + r * D + 32 * m + 2 * e + 4 * half) =
+                f32x4_t{O[m][e], O[m][e + 1], O[m][e + 2], O[m][e + 3]};
+        if (half == 0) {
+          slot[32 * WAVES * D + r] = M;
+          slot[32 * WAVES * (D + 1) + r] = sum;
+        }
+      }
+    } else {
+      // a row that sees no token gives zeros
+      const float inv = seen >= 0 || sum != sum ? 1.f / sum : 0.f;
+      uint16_t* o = p.out + (((int64_t)sq.row0 + token) * p.heads + head) * D + 4 * half;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<f32x4_t*>(slot + r * D + 32 * m + 2 * e + 4 * half) =
-              f32x4_t{O[m][e], O[m][e + 1], O[m][e + 2], O[m][e + 3]};
-      if (half == 0) {
-        slot[32 * WAVES * D + r] = M;
-        slot[32 * WAVES * (D + 1) + r] = sum;
-      }
+          if (mine)
+            *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) =
+                u32x2_t{result_pair<BF>(O[m][e] * inv, O[m][e + 1] * inv),
+                        result_pair<BF>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
     }
-    return;
   }
-  // a row that sees no token gives zeros
-  const float inv = seen >= 0 || sum != sum ? 1.f / sum : 0.f;
-  uint16_t* o = p.out + (((int64_t)sq.row0 + token) * p.heads + head) * D + 4 * half;
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      if (mine)
-        *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) =
-            u32x2_t{result_pair<BF>(O[m][e] * inv, O[m][e + 1] * inv),
-                    result_pair<BF>(O[m][e + 2] * inv, O[m][e + 3] * inv)};
+  x += part;
+  if constexpr (PIECES)
+    if (x < end) {
+      mine_of_lane = chunk_sequence(p.batch, lane - 1);  // again, and not kept through the products
+      __syncthreads();                                   // the tiles in LDS have been read
+    }
+  }
 }
 
-// Joins the runs of split units, 1024 results at a time, 4 per thread.  Whether there
-// are any only the device knows, so that few blocks are launched, which take them in turn.
+// Joins the parts of units that were split or cut, 1024 results at a time, 4 per thread; those of
+// a unit that was cut by the first end of a block's piece inside of it.  How many there are
+// only the device knows, so that few blocks are launched, which take them in turn.
 constexpr int kJoinBlocks = 2048;
-template <bool BF, int D>
+template <bool BF, int D, bool PIECES>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkParams p) {
   constexpr int ROWS = 1024 / D;
   const int block_rows = p.batch.block_rows, parts = block_rows / ROWS, per = p.batch.per;
   const int lane = threadIdx.x & 63, c = threadIdx.x % (D / 4) * 4;
-  ChunkShare share;
-  for (int id = blockIdx.x; find_chunk(p.batch, id / parts, true, lane, share); id += kJoinBlocks) {
+  ChunkSequence mine_of_lane;
+  Line line;
+  if constexpr (PIECES) {
+    mine_of_lane = chunk_sequence(p.batch, lane - 1);
+    line = line_of(p.batch, mine_of_lane, lane);
+    if (!line.pieces) return;
+  }
+  for (int id = blockIdx.x;; id += kJoinBlocks) {
+    ChunkSequence sq;
+    int block, kvh, runs, place;
+    bool second = false;  // the first part is the second one of its block
+    if constexpr (PIECES) {
+      const int cut = id / parts + 1;  // the end of block cut - 1
+      if ((int64_t)cut * line.width >= line.total) return;
+      Piece share;
+      if (!find_piece(p.batch, line, mine_of_lane, cut * line.width, lane, share)) return;
+      if (share.at == 0 || share.at > line.width) continue;
+      sq = share.q;
+      block = share.block;
+      kvh = share.head;
+      runs = (share.length - share.at + line.width - 1) / line.width + 1;
+      place = 2 * (cut - 1);
+      second = share.at < line.width;
+      if (place + 2 * (runs - 1) >= p.batch.pieces) continue;  // offsets that are not ascending
+    } else {
+      ChunkShare share;
+      if (!find_chunk(p.batch, id / parts, true, lane, share)) return;
+      sq = share.q;
+      block = share.block;
+      kvh = share.head;
+      runs = share.runs;
+      place = (int)share.slot;
+    }
     const int r = id % parts * ROWS + threadIdx.x / (D / 4);
-    const int row = share.block * block_rows + r;
-    if (row >= share.q.rows * per) continue;
-    const int token = quotient(row, per, p.batch.per_shift), head = share.head * per + row - token * per;
-    const float* slot = p.partial + share.slot * p.slot;
-    const int64_t step = p.slot;
+    const int row = block * block_rows + r;
+    if (row >= sq.rows * per) continue;
+    const int token = quotient(row, per, p.batch.per_shift), head = kvh * per + row - token * per;
+    auto slot_of = [&](int i) {
+      return p.partial + (int64_t)(place + (PIECES ? 2 * i + (i == 0 && second ? 1 : 0) : i)) * p.slot;
+    };
     float M = kLow, sum = 0.f;
-    for (int i = 0; i < share.runs; ++i) M = fmaxf(M, slot[i * step + block_rows * D + r]);
+    for (int i = 0; i < runs; ++i) M = fmaxf(M, slot_of(i)[block_rows * D + r]);
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = 0; i < share.runs; ++i) {
-      const float f = __builtin_amdgcn_exp2f(slot[i * step + block_rows * D + r] - M);
-      sum = fmaf(f, slot[i * step + block_rows * (D + 1) + r], sum);
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(slot + i * step + r * D + c);
+    for (int i = 0; i < runs; ++i) {
+      const float* slot = slot_of(i);
+      const float f = __builtin_amdgcn_exp2f(slot[block_rows * D + r] - M);
+      sum = fmaf(f, slot[block_rows * (D + 1) + r], sum);
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(slot + r * D + c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, v[e], o[e]);
     }
-    const bool sees = token + share.q.length - share.q.rows >= 0;
+    const bool sees = token + sq.length - sq.rows >= 0;
     const float inv = sees || sum != sum ? 1.f / sum : 0.f;
-    *reinterpret_cast<u32x2_t*>(p.out + (((int64_t)share.q.row0 + token) * p.heads + head) * D + c) =
+    *reinterpret_cast<u32x2_t*>(p.out + (((int64_t)sq.row0 + token) * p.heads + head) * D + c) =
         u32x2_t{result_pair<BF>(o[0] * inv, o[1] * inv), result_pair<BF>(o[2] * inv, o[3] * inv)};
   }
 }
@@ -532,18 +728,16 @@ ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int 
   ChunkPlan plan = {};
   plan.few_rows = all <= 512 ? 256 : all <= 2048 ? 128 : 64;
   const bool few = rows <= plan.few_rows * seqs, both = !few && seqs > 1 && per <= plan.few_rows;
-  auto fill = [&](ChunkPart& part, int64_t units, int most) {
-    const int64_t longest = ((capacity + part.tile - 1) / part.tile + part.least - 1) / part.least;
+  auto reserve = [&](ChunkPart& part, int64_t units, int pieces) {
     part.units = units;
-    part.most = (int)(longest < 1 ? 1 : longest < most ? longest : most);
-    const int64_t more = units * (part.most - 1);
-    part.grid = units + (more < part.blocks ? more : part.blocks);
     part.slot = (int64_t)part.block_rows * (head_size + 2);
+    part.pieces = part.most == 1 ? 0 : pieces;
     if (part.most == 1) return;
     if (plan.workspace == 0) plan.workspace = kKv4Counters * sizeof(uint32_t);
     part.partial = plan.workspace;
-    plan.workspace += ((size_t)(part.blocks * part.slot) * sizeof(float) + 255) / 256 * 256;
+    plan.workspace += ((size_t)pieces * part.slot * sizeof(float) + 255) / 256 * 256;
   };
+  const int64_t most_tiles = (capacity + kKeys - 1) / kKeys;
   // a partial block for every sequence and for the rows in front of them and behind
   auto units_of = [&](int64_t block_rows) { return ((rows + block_rows - 1) / block_rows + seqs + 2) * kv_heads; };
   if (few || both) {
@@ -558,7 +752,11 @@ ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int 
     // Of a few thousand tokens (8 sequences of 3000, 2 tokens each: 15.8 us with 16 steps, 18.0
     // with 32); short ones are not split (32 of 600: 11.5, 9.9 unsplit).
     plan.few.least = 16;
-    fill(plan.few, units, units <= kKv4Counters ? 256 : 1);
+    const int64_t longest = (capacity + 31) / 32 / plan.few.least;
+    plan.few.most = units > kKv4Counters || longest < 2 ? 1 : longest < 256 ? (int)longest : 256;
+    const int64_t more = units * (plan.few.most - 1);
+    plan.few.grid = units + (more < plan.few.blocks ? more : plan.few.blocks);
+    reserve(plan.few, units, plan.few.blocks);
   }
   if (!few) {
     plan.tiles.waves = head_size > 128 ? 4 : 8;
@@ -567,7 +765,17 @@ ChunkPlan plan_chunk(int64_t tokens, int64_t seqs, int heads, int kv_heads, int 
     plan.tiles.blocks = 256;
     plan.tiles.least = 8;
     const int64_t units = units_of(plan.tiles.block_rows);
-    fill(plan.tiles, units, units < 4 * plan.tiles.blocks ? 64 : 1);
+    // four rounds of blocks are even enough by themselves
+    const bool cut = units < 4 * plan.tiles.blocks && most_tiles > plan.tiles.least && units * most_tiles < 1 << 26;
+    // equal pieces where a block has some 48 tiles: finding them takes 10 us
+    const int64_t tiles = (rows + plan.tiles.block_rows - 1) / plan.tiles.block_rows * kv_heads * most_tiles;
+    const bool pieces = cut && tiles >= 48 * plan.tiles.blocks;
+    const int64_t longest = most_tiles / plan.tiles.least;
+    plan.tiles.most = !cut || longest < 2 ? 1 : longest < 64 ? (int)longest : 64;
+    const int64_t more = plan.tiles.most == 1 ? 0 : plan.tiles.blocks;
+    plan.tiles.grid = pieces ? (units > plan.tiles.blocks ? units : plan.tiles.blocks) : units + more;
+    reserve(plan.tiles, units, (pieces ? 2 : 1) * plan.tiles.blocks);
+    if (!pieces) plan.tiles.pieces = 0;
   }
   return plan;
 }
@@ -578,8 +786,11 @@ int launch_chunk_attention(const ChunkParams& p, int dtype, hipStream_t st) {
   auto go = [&](auto bf, auto d) -> int {
     constexpr bool BF = decltype(bf)::value;
     constexpr int D = decltype(d)::value, WAVES = D > 128 ? 4 : 8;
-    hipLaunchKernelGGL((chunk_attention_kernel<BF, D, WAVES>), dim3((uint32_t)p.grid), dim3(64 * WAVES), 0, st, p);
-    if (split) hipLaunchKernelGGL((chunk_join_kernel<BF, D>), dim3(kJoinBlocks), dim3(256), 0, st, p);
+    const bool pieces = p.batch.pieces > 0;
+    auto kernel = pieces ? chunk_attention_kernel<BF, D, WAVES, true> : chunk_attention_kernel<BF, D, WAVES, false>;
+    auto join = pieces ? chunk_join_kernel<BF, D, true> : chunk_join_kernel<BF, D, false>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)p.grid), dim3(64 * WAVES), 0, st, p);
+    if (split) hipLaunchKernelGGL(join, dim3(kJoinBlocks), dim3(256), 0, st, p);
     return hipGetLastError() == hipSuccess ? GRINQH_OK : GRINQH_ERR_HIP;
   };
   auto sized = [&](auto bf) -> int {

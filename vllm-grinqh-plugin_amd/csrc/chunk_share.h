@@ -29,6 +29,17 @@ __device__ __forceinline__ ChunkSequence chunk_sequence(const ChunkBatch& b, int
 // x / d for x >= 0, d > 0; shift: log2(d) where d is a power of two, otherwise negative.
 __device__ __forceinline__ int quotient(int x, int d, int shift) { return shift >= 0 ? x >> shift : x / d; }
 
+// Blocks of rows of sequence s that this kernel takes, and tiles of its tokens.
+__device__ __forceinline__ int chunk_blocks(const ChunkBatch& b, const ChunkSequence& q, int s) {
+  const int64_t rows = (int64_t)q.rows * b.per;
+  const bool edge = s < 0 || s >= b.seqs;
+  if (edge ? !b.edges : rows < b.least_rows || rows > b.most_rows) return 0;
+  return (int)((rows + b.block_rows - 1) >> b.rows_shift);
+}
+__device__ __forceinline__ int chunk_tiles(const ChunkBatch& b, const ChunkSequence& q) {
+  return (int)(((int64_t)q.length + b.tile - 1) >> b.tile_shift);
+}
+
 struct ChunkShare {
   ChunkSequence q;
   int seq, head;   // key/value head
@@ -43,17 +54,12 @@ struct ChunkShare {
 // key/value head, and the tiles of b.tile tokens that they read are shared out over
 // b.blocks: a unit is split into as many runs as it has shares of at least b.least
 // tiles, all units of a sequence alike, so that split units have b.blocks runs at most
-// and a batch with fewer units than that runs in one round.  With `joined` blocks
-// stand for split units.  False: past the last one.
+// and a batch with fewer units than that runs in one round.  With `joined` blocks stand
+// for split units.  False: past the last one.
 __device__ __forceinline__ bool find_chunk(const ChunkBatch& b, int64_t id, bool joined, int lane, ChunkShare& out) {
   const int heads = b.kv_heads;
-  auto blocks_of = [&](const ChunkSequence& q, int s) {
-    const int64_t rows = (int64_t)q.rows * b.per;
-    const bool edge = s < 0 || s >= b.seqs;
-    if (edge ? !b.edges : rows < b.least_rows || rows > b.most_rows) return 0;
-    return (int)((rows + b.block_rows - 1) >> b.rows_shift);
-  };
-  auto tiles_of = [&](const ChunkSequence& q) { return (int)(((int64_t)q.length + b.tile - 1) >> b.tile_shift); };
+  auto blocks_of = [&](const ChunkSequence& q, int s) { return chunk_blocks(b, q, s); };
+  auto tiles_of = [&](const ChunkSequence& q) { return chunk_tiles(b, q); };
   // the first 64 are looked at once
   ChunkSequence q = {0, 0, 0, false};
   if (lane - 1 <= b.seqs) q = chunk_sequence(b, lane - 1);
