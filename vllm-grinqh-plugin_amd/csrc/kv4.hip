@@ -377,6 +377,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 2 : 3) void kv4_attention_ker
   if constexpr (CHUNK) {
     ChunkShare share;
     if (!find_chunk(batch, blockIdx.x, false, lane, share)) return;
+    // offsets that are not ascending: runs that no block takes would be waited for
+    if (share.runs > 1 && (int64_t)blockIdx.x - share.run + share.runs > gridDim.x) return;
     const int all = share.q.rows * per;
     row0 = share.block * kRows;
     rows = min(kRows, all - row0);
