@@ -493,10 +493,15 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   RawValues<D, WAVES> values;
   // One tile: its weights and its part of O, and the products of the next tile, slot by
   // slot: every slot gives the matrix unit one product and the vector unit a share
-  // of the exponentials and of the unpacking (keys two tiles ahead, values one).
-  constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = 3;
+  // of the exponentials and, under the keys' products, of the unpacking (keys two tiles
+  // ahead, values one).  What was unpacked makes room for the next loads, which then have
+  // more than half a tile's time to arrive (1 sequence of 32768 tokens, 2048 rows, 32 heads of
+  // 128: 1080 us, 1140 with loads at the tile's end).  Heads of 256 channels have no registers
+  // for that: their values are unpacked under the values' products.
+  constexpr bool EARLY = D <= 128;
+  constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = PIECES && D == 128 ? 2 : 3, SETTLE = KSLOTS / 4;
   auto step = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], const uint8_t* kt, const uint8_t* vt, uint8_t* k_to, uint8_t* v_to,
-                  float& top) {
+                  float& top, auto&& refill) {
     u32x4_t f[AHEAD + 1];
     auto read = [&](int at) {  // the A operand of slot `at`
       f[at % (AHEAD + 1)] =
@@ -504,19 +509,31 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
     };
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) read(k);
-    settle_raw(keys, values);
+    if constexpr (!EARLY) settle_raw(keys, values);
     int done = 0, packed = 0;
 #pragma unroll
     for (int k = 0; k < KSLOTS; ++k) {
       const int b = k / STEPS, s = k % STEPS;
+      if (EARLY && k == SETTLE) settle_raw(keys, values);
       read(k + AHEAD);
       N[b] = mfma32x32x16(f[k % (AHEAD + 1)], qf[s], s == 0 ? (f32x16_t)(0.f) : N[b]);
 #pragma unroll
       for (; done < (k + 1) * 8 / KSLOTS; ++done) weigh(S, 0, done);
+      if constexpr (EARLY) {
 #pragma unroll
-      for (; packed < (k + 1) * R::WORDS / KSLOTS; ++packed) write_key(keys, packed, k_to);
+        for (; k >= SETTLE && packed < (k + 1 - SETTLE) * 2 * R::WORDS / (KSLOTS - SETTLE); ++packed) {
+          if (packed < R::WORDS)
+            write_key(keys, packed, k_to);
+          else
+            write_value(values, packed - R::WORDS, v_to);
+        }
+      } else {
+#pragma unroll
+        for (; packed < (k + 1) * R::WORDS / KSLOTS; ++packed) write_key(keys, packed, k_to);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (EARLY) refill();
     done = packed = 0;
     int seen_of = 0;
     top = -__builtin_inff();
@@ -533,8 +550,10 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
         for (; seen_of < (k + 1 - VSLOTS / 2) * 16 / (VSLOTS / 2); ++seen_of)
           top = fmaxf(fmaxf(top, N[seen_of >> 3][2 * (seen_of & 7)]), N[seen_of >> 3][2 * (seen_of & 7) + 1]);
       }
+      if constexpr (!EARLY) {
 #pragma unroll
-      for (; packed < (k + 1) * R::WORDS / VSLOTS; ++packed) write_value(values, packed, v_to);
+        for (; packed < (k + 1) * R::WORDS / VSLOTS; ++packed) write_value(values, packed, v_to);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -583,17 +602,21 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   }
   auto turn = [&](f32x16_t (&S)[2], f32x16_t (&N)[2], int j, int at) {  // at: j - first is odd
     __syncthreads();
+    auto refill = [&]() {
+      load_values(values, j + 2, page_before);
+      load_keys(keys, j + 3, page);
+      page_before = page;
+      page = page_of(j + 4);
+    };
     if (j < my_last) {
-      step(S, N, s_k[at ^ 1], s_v[at], s_k[at], s_v[at ^ 1], top);
+      step(S, N, s_k[at ^ 1], s_v[at], s_k[at], s_v[at ^ 1], top, refill);
     } else {
       settle_raw(keys, values);
       feed_keys(s_k[at]);
       feed_values(s_v[at ^ 1]);
+      if constexpr (EARLY) refill();
     }
-    load_values(values, j + 2, page_before);
-    load_keys(keys, j + 3, page);
-    page_before = page;
-    page = page_of(j + 4);
+    if constexpr (!EARLY) refill();
     if (j + 1 < my_last) settle(N, top, j + 1);
   };
   for (int j = first; j < last; j += 2) {
