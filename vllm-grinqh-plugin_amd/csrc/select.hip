@@ -9,6 +9,11 @@
 // times powers of two, so nothing is rounded and the selection does not depend on
 // the order of any sum.  The means are sums in 64 bits that are exact too: what a code
 // stands for is a multiple of 2^-24 below 2^17, and 4096 tokens of it fit 53 bits.
+//
+// All are bound by latency: of a page's records (summaries: 32 tokens' pages 4.7 us, 4
+// prompts of 2048 tokens 7.4 us, 0.8 TB/s), of the search for the last selected score.
+// 64 sequences of 8192 tokens, pages of 16, 8 key/value heads of 128: 16 us, 38 MB of
+// summaries; one of 131072 tokens, 9.4 MB: 5 us for the scores, 14 for the search.
 #include <cfloat>
 #include <type_traits>
 
@@ -546,8 +551,11 @@ __global__ __launch_bounds__(THREADS) void kv4_top_kernel(const SelectParams p) 
       [&](int j, int place) { out[place] = PER > 0 ? index[PER > 0 ? j : 0] : table[first + j]; });
 }
 
-// Both in one launch.
-constexpr int kSelectPages = 2048;
+// Both in one launch, up to 1024 pages. As two (1, 8, 64 sequences, 8 key/value heads of
+// 128, us): 512 pages 8.1, 8.2, 16.0 in one and 8.7, 9.0, 19.8 in two; 1024: 10.9, 11.1, 26
+// and 8.8, 9.3, 30; 2047: 17.2, 18.7, 47 and 9.2, 11.4, 38. The second of the two has 2, 8 or any
+// number of pages per thread (2047 pages with 8: 12.8, 15.0, 44).
+constexpr int kSelectPages = 1024;
 template <typename DT, int D>
 __global__ __launch_bounds__(kThreads, 4) void kv4_select_kernel(const SelectParams p) {
   constexpr int PER = kSelectPages / kThreads;
@@ -623,7 +631,9 @@ int launch_kv4_select(const SelectParams& p, int dtype, hipStream_t st) {
     });
     if (s != GRINQH_OK) return s;
   }
-  if (p.table_width <= 8192)
+  if (p.table_width <= 2048)
+    hipLaunchKernelGGL((kv4_top_kernel<1024, 2>), units, dim3(1024), 0, st, p);
+  else if (p.table_width <= 8192)
     hipLaunchKernelGGL((kv4_top_kernel<1024, 8>), units, dim3(1024), 0, st, p);
   else
     hipLaunchKernelGGL((kv4_top_kernel<1024, 0>), units, dim3(1024), 0, st, p);
