@@ -6,6 +6,33 @@
 // Rows of a block are (token, query head of one key/value head) pairs, so that all
 // heads that share keys share the work of unpacking them: a tile of 64 tokens is
 // loaded as it is kept, turned into fp16 by all threads together and left in LDS.
+//
+// A wave has 32 rows.  S^T = K Q^T and O^T = V^T P^T with 32x32x16 matrix instructions: a
+// lane then holds one row's logits, so that its maximum and sum need one exchange with
+// lane + 32, and the weights are the second product's operand as they come out (the
+// values are read transposed, whose order of tokens is the logits').  The reference that
+// is taken off the logits is raised only where a weight would pass 2^8, so most tiles
+// leave O alone.
+//
+// Precision: queries are brought to 2^13 <= max < 2^14 by a power of two and rounded to fp16
+// (exact unless a row spans more than fp16 holds); keys and values are rounded to fp16
+// once, minimum + scale * code in one fused operation; weights to fp16 after the sum has
+// taken the rounded ones.  Logits, references, sums and O are fp32.  Against 64 bits, fp16
+// tensors, relative in the norm: 4.8e-4, which is half a step of the type (the results' own
+// rounding is 2.1e-4 of that, and the single-token kernel, whose codes are exact, has
+// 2.9e-4); bf16 tensors: 1.7e-3, their rounding alone.
+//
+// Bound by the vector unit's work for every token beside the products (2048 rows, a
+// sequence of 32768 tokens, 32 query and 8 key/value heads of 128, 1065 GFLOP: 1080 us, 980
+// TFLOP/s, a large library product reaches 1300; matrix unit 47 % of the cycles, vector unit
+// 49, LDS 32, at the 1.77 GHz that the card holds under this load).  32768 tokens are
+// unpacked by 32 blocks of each head again, an eighth of the vector unit's time; the
+// exponentials and the rounding to fp16 are the rest.  256 rows share a tile: with 128, two
+// blocks to a CU, 819 TFLOP/s instead of 917 (of an earlier version of both).  Heads of 256
+// channels have registers for one wave per SIMD and 128 rows, so that nothing runs
+// beside a wave that waits (2 sequences of 2500 tokens, 700 rows, 16 and 8 heads: 163 us, 400
+// TFLOP/s, matrix unit 16 % of the cycles; 176 units on 256 CUs, and the longest of 40 tiles
+// takes all that time).
 #include <cfloat>
 #include <type_traits>
 
