@@ -204,17 +204,17 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         stream = _stream(dev.index)
         nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
         ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
-        lib, space = _lib.load_library(), (ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
+        at, room = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
         if table_head is None:
-            _lib.check(lib.grinqh_kv4_attention(
+            _lib.check(_lib.load_library().grinqh_kv4_attention(
                 q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
                 page_table.data_ptr(), table_stride, width, lengths.data_ptr(), _scale(scale, d), out.data_ptr(), dt,
-                *space, stream), "grinqh_kv4_attention")
+                at, room, stream), "grinqh_kv4_attention")
         else:
-            _lib.check(lib.grinqh_kv4_attention_selected(
+            _lib.check(_lib.load_library().grinqh_kv4_attention_selected(
                 q.data_ptr(), q_token, q_head, seqs, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
                 page_table.data_ptr(), table_stride, table_head, width, lengths.data_ptr(), _scale(scale, d),
-                out.data_ptr(), dt, *space, stream), "grinqh_kv4_attention_selected")
+                out.data_ptr(), dt, at, room, stream), "grinqh_kv4_attention_selected")
     return out
 
 
