@@ -136,3 +136,36 @@ def test_two_graphs_at_once_and_eager_calls_between(rows):
         eager = ga.kv4_chunk_attention(q, cache, wide, lengths, ends)
         torch.cuda.synchronize()
         assert all(torch.equal(x, want) for x in (*outs, eager))
+
+
+def test_tables_without_pages():
+    """no room for any token: rows see none, and a length is past the table"""
+    from grinqh import attention as ga
+    cache, table, lengths, kv, q, ends = _chunk_case(5, [40, 40], [3, 200], 2, 4, 128, 16, 64, "f16")
+    for x, e in ((q, ends), (q[:5], _i32([0, 3, 5]))):
+        assert not ga.kv4_chunk_attention(x, cache, table[:, :0], lengths * 0, e).any()
+        assert bool(ga.kv4_chunk_attention(x, cache, table[:, :0], lengths, e).isnan().all())
+
+
+@pytest.mark.parametrize("per,d", [(65, 64), (128, 128), (130, 256)])
+def test_more_heads_per_key_head_than_rows_of_a_block(per, d):
+    """one token is more rows than the single-token kernel or the tile kernel takes in a block"""
+    from grinqh import attention as ga
+    lens, news = [300, 5, 1, 70], [1, 5, 1, 9]
+    cache, table, lengths, kv, q, ends = _chunk_case(per, lens, news, 1, per, d, 16, d, "bf16")
+    for tab in (table, _wide(table)):
+        _check_chunk(ga.kv4_chunk_attention(q, cache, tab, lengths, ends), q, kv, news, d, "bf16")
+
+
+@pytest.mark.parametrize("new", [2, 90])
+def test_sequences_that_share_pages(new):
+    """one prefix, several questions: the same pages in several rows of the table"""
+    from grinqh import attention as ga
+    case = _chunk_case(new, [400], [new], 2, 4, 128, 16, 64, "f16")
+    cache, table, lengths, kv, q, ends = case
+    want = ga.kv4_chunk_attention(q, cache, _wide(table), lengths, ends)
+    _check_chunk(want, q, kv, [new], 64, "f16")
+    n = 5
+    out = ga.kv4_chunk_attention(q.repeat(n, 1, 1), cache, _wide(table).expand(n, -1), lengths.expand(n),
+                                 _i32(np.arange(n + 1) * new))
+    _check_chunk(out, q.repeat(n, 1, 1), kv * n, [new] * n, 64, "f16")

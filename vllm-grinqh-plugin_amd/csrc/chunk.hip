@@ -23,11 +23,11 @@
 // 2.9e-4); bf16 tensors: 1.7e-3, their rounding alone.
 //
 // Bound by the vector unit's work for every token beside the products (2048 rows, a
-// sequence of 32768 tokens, 32 query and 8 key/value heads of 128, 1065 GFLOP: 1080 us, 980
+// sequence of 32768 tokens, 32 query and 8 key/value heads of 128, 1065 GFLOP: 1090 us, 975
 // TFLOP/s, a large library product reaches 1300; matrix unit 47 % of the cycles, vector unit
-// 49, LDS 32, at the 1.77 GHz that the card holds under this load).  32768 tokens are
-// unpacked by 32 blocks of each head again, an eighth of the vector unit's time; the
-// exponentials and the rounding to fp16 are the rest.  256 rows share a tile: with 128, two
+// 49, LDS 32, at the 1.77 GHz that the card holds under this load).  The tokens are unpacked
+// by each of a head's 32 blocks of rows, 13 instructions for 8 codes or about a fifth of the
+// vector unit's; the exponentials, their sums and their rounding are most of the rest.  256 rows share a tile: with 128, two
 // blocks to a CU, 819 TFLOP/s instead of 917 (of an earlier version of both).  Heads of 256
 // channels have registers for one wave per SIMD and 128 rows, so that nothing runs
 // beside a wave that waits (2 sequences of 2500 tokens, 700 rows, 16 and 8 heads: 163 us, 400
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   // of the exponentials and, under the keys' products, of the unpacking (keys two tiles
   // ahead, values one).  What was unpacked makes room for the next loads, which then have
   // more than half a tile's time to arrive (1 sequence of 32768 tokens, 2048 rows, 32 heads of
-  // 128: 1080 us, 1140 with loads at the tile's end).  Heads of 256 channels have no registers
+  // 128: 1085 us, 1140 with loads at the tile's end).  Heads of 256 channels have no registers
   // for that: their values are unpacked under the values' products.
   constexpr bool EARLY = D <= 128;
   constexpr int KSLOTS = 2 * STEPS, VSLOTS = 4 * MT, AHEAD = PIECES && D == 128 ? 2 : 3, SETTLE = KSLOTS / 4;
