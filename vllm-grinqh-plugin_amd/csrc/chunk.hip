@@ -16,8 +16,8 @@
 //
 // Precision: queries are brought to 2^13 <= max < 2^14 by a power of two and rounded to fp16
 // (exact unless a row spans more than fp16 holds); keys and values are rounded to fp16
-// once, minimum + scale * code in one fused operation; weights to fp16 after the sum has
-// taken the rounded ones.  Logits, references, sums and O are fp32.  Against 64 bits, fp16
+// once, minimum + scale * code in one fused operation; weights to fp16, and summed as
+// rounded.  Logits, references, sums and O are fp32.  Against 64 bits, fp16
 // tensors, relative in the norm: 4.8e-4, which is half a step of the type (the results' own
 // rounding is 2.1e-4 of that, and the single-token kernel, whose codes are exact, has
 // 2.9e-4); bf16 tensors: 1.7e-3, their rounding alone.
@@ -27,8 +27,9 @@
 // TFLOP/s, a large library product reaches 1300; matrix unit 47 % of the cycles, vector unit
 // 49, LDS 32, at the 1.77 GHz that the card holds under this load).  The tokens are unpacked
 // by each of a head's 32 blocks of rows, 13 instructions for 8 codes or about a fifth of the
-// vector unit's; the exponentials, their sums and their rounding are most of the rest.  256 rows share a tile: with 128, two
-// blocks to a CU, 819 TFLOP/s instead of 917 (of an earlier version of both).  Heads of 256
+// vector unit's; the exponentials, their sums and their rounding are most of the rest.
+// 256 rows share a tile: with 128, two blocks to a CU, 819 TFLOP/s instead of 917 (of an
+// earlier version of both).  Heads of 256
 // channels have registers for one wave per SIMD and 128 rows, so that nothing runs
 // beside a wave that waits (2 sequences of 2500 tokens, 700 rows, 16 and 8 heads: 163 us, 400
 // TFLOP/s, matrix unit 16 % of the cycles; 176 units on 256 CUs, and the longest of 40 tiles
