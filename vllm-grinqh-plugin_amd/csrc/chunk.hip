@@ -11,13 +11,16 @@
 // lane then holds one row's logits, so that its maximum and sum need one exchange with
 // lane + 32, and the weights are the second product's operand as they come out (the
 // values are read transposed, whose order of tokens is the logits').  The reference that
-// is taken off the logits is raised only where a weight would pass 2^8, so most tiles
-// leave O alone.
+// is taken off the logits is raised only where a weight would pass 2^15, so most tiles
+// leave O alone; it then is 7 below the largest logit (kRoom).
 //
 // Precision: queries are brought to 2^13 <= max < 2^14 by a power of two and rounded to fp16
 // (exact unless a row spans more than fp16 holds); keys and values are rounded to fp16
 // once, minimum + scale * code in one fused operation; weights to fp16, and summed as
-// rounded.  Logits, references, sums and O are fp32.  Against 64 bits, fp16
+// rounded.  A row's largest weight is between 2^7 and 2^15, so weights are normal fp16 numbers
+// down to 2^-21 of it, and off by 2^-32 of it at most below: with one token above 32768 others by
+// 17 nats, its value near zero, results are as exact as any (with the largest weight at 1 they were
+// 3e-2 off).  Logits, references, sums and O are fp32.  Against 64 bits, fp16
 // tensors, relative in the norm: 4.8e-4, which is half a step of the type (the results' own
 // rounding is 2.1e-4 of that, and the single-token kernel, whose codes are exact, has
 // 2.9e-4); bf16 tensors: 1.7e-3, their rounding alone.
@@ -52,6 +55,9 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_t;
 
 constexpr int kKeys = 64;         // tokens per tile
 constexpr float kLow = -FLT_MAX;  // running reference before the first token (finite: -inf - -inf would be NaN)
+// A raised reference is so far below the largest logit that its weight is 2^7, and one that would pass 2^15 raises it
+// again.  Less than 8, half of fp32's step at 2^27: the difference is rounded to one step at most there, and to none beyond.
+constexpr float kRoom = 7.f, kRaise = 15.f;
 
 __device__ __forceinline__ f32x16_t mfma32x32x16(const u32x4_t& a, const u32x4_t& b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0,
@@ -472,7 +478,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
     return top;
   };
   // Makes S of a tile ready for its weights: the mask where the tile reaches past the
-  // wave's first row's last token, and the reference raised where a weight would pass 2^8.
+  // wave's first row's last token, and the reference raised where a weight would pass 2^15.
   auto settle = [&](f32x16_t (&S)[2], float top, int tile) {
     if (tile * kKeys + kKeys - 1 > wave_seen) {
       asm volatile("");  // a branch: as selects, this is a fourth of every tile's instructions
@@ -489,14 +495,14 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
       product_first(S);
       top = largest(S);
     }
-    if (__any(fmaf(top, zs, -M) > 8.f)) {
-      float m = fmaxf(M, top * zs);
+    if (__any(fmaf(top, zs, -M) > kRaise)) {
+      float m = fmaxf(M, top * zs - kRoom);
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       if (!far && __any(fabsf(m) > 0x1p24f && m != kLow)) {
         far = true;
         zs = 1.f;
         product_first(S);
-        m = fmaxf(M, largest(S));
+        m = fmaxf(M, largest(S) - kRoom);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
       }
       const float f = __builtin_amdgcn_exp2f(M - m);
@@ -507,8 +513,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
     }
   };
   u32x4_t P[4];
-  // Weights of two tokens, pair q of key block b, as fp16 for the second product (2^-11 of
-  // them at most); they are summed as rounded, in fp32.
+  // Weights of two tokens, pair q of key block b, as fp16 for the second product (off by 2^-11 of
+  // them, or by 2^-25 below 2^-14); they are summed as rounded, in fp32.
   auto weigh = [&](const f32x16_t (&S)[2], int b, int q) {
     const float p0 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q], zs, -M));
     const float p1 = __builtin_amdgcn_exp2f(fmaf(S[b][2 * q + 1], zs, -M));
