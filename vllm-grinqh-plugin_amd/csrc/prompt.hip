@@ -75,6 +75,14 @@ constexpr int kKeys = 64;       // keys per tile
 // running reference before the first key (finite: -inf - -inf would be NaN; a row of
 // logits below it is one for the second pass)
 constexpr float kLow = -1e30f;
+// A raised reference is so far (in powers of two) below the largest logit, and is raised again where a weight would
+// pass 2^kRaise.  fp16's weights need that room below: beside a largest one of 1, those 17 nats lower are subnormal or
+// zero, and where they are many thousands, of a token with a value near zero and all others, results were 3e-2 off.  From
+// 2^7 on they are normal numbers down to 2^-21 of the largest, and off by 2^-32 of it below.  bf16 has the range.
+template <typename DT>
+constexpr float kRoom = DT::id == F16::id ? 7.f : 0.f;
+template <typename DT>
+constexpr float kRaise = kRoom<DT> + 8.f;
 
 // A value that all lanes agree on, in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -303,7 +311,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
     };
     // Makes S of a tile ready for its weights: the mask where the tile reaches
     // past a row's last key, and the reference raised where a weight would pass
-    // 2^8 (rarely after the first tiles: the accumulators are not rescaled for less).
+    // 2^kRaise (rarely after the first tiles: the accumulators are not rescaled for less).
+    // With `far` it is the largest logit itself, whose steps are wider than the room.
     auto settle = [&](f32x16_t (&S)[2], float& top, int tile) {
       if (tile * kKeys + kKeys - 1 > row0 + shift) {
         // last key of this tile that the row sees, less the half's 4 (compared with constants)
@@ -317,8 +326,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
             top = fmaxf(top, S[b][e]);
           }
       }
-      if (__any(power(top) > 8.f)) {
-        float m = fmaxf(M, APART && far ? top : top * c2);
+      if (__any(power(top) > kRaise<DT>)) {
+        float m = fmaxf(M, APART && far ? top : top * c2 - kRoom<DT>);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float f = __builtin_amdgcn_exp2f(APART && far ? (M - m) * c2 : M - m);
         M = m;
@@ -488,8 +497,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void prompt_attention
         if (row < rows) *reinterpret_cast<u32x2_t*>(o + 32 * m + 2 * e) = w;
       }
     if (APART || tiles == 0) return 0;
-    // A row's largest weight is 1 or more, where its exponent was right.
-    const bool lost = l < 0.5f && row < rows && row + shift >= 0;
+    // A row's largest weight is 2^kRoom or more, where its exponent was right.
+    const bool lost = l < 0.5f * (float)(1 << (int)kRoom<DT>) && row < rows && row + shift >= 0;
     int mine = 0;
     if (__any(odd != odd || lost)) mine = __any(lost || fabsf(M) > 0x1p24f && M != kLow) ? kApart | kFar : kApart;
     if (lane == 0) s_redo[wave] = mine;
