@@ -369,9 +369,10 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void chunk_attention_k
   };
   // A token whose values are NaN (or lie outside the cache) gives zeros, and NaN as
   // its key: that reaches the rows that see it and no others, as the others' logits are
-  // masked.  So does what no token was stored as, which stands behind a sequence's end and
-  // must only stay finite.  All that takes one test in most tiles.
-  auto beyond = [](uint32_t pair) { return !(fabsf(reach_of(pair)) <= 65568.f); };
+  // masked.  So does what no token was stored as, its largest code past what fp16 holds to either
+  // side: it stands behind a sequence's end and must only stay finite.  All that takes one
+  // test in most tiles.
+  auto beyond = [](uint32_t pair) { return !(fabsf(reach_of(within(pair))) <= 65504.f); };
   auto settle_keys = [&](RawKeys<D, WAVES>& k) {
 #pragma unroll
     for (int i = 0; i < R::PAIRS; ++i) k.pair[i] = k.lost || beyond(k.value_pair) ? 0x7E007E00u : within(k.pair[i]);
