@@ -234,11 +234,13 @@ int grinqh_kv4_load(const void* cache, int64_t pages, int kv_heads, int page_siz
  * lengths are read on the device, where the blocks share the work out.  The
  * workspace (grinqh_kv4_attention_workspace_bytes for a capacity of table_width *
  * page_size tokens, 256-byte aligned) is zero-filled once before its first use
- * (every call leaves its counters zero again); calls that share one must be
- * ordered (same stream).  Its size grows with seqs up to 1024 sequences and
+ * (every call leaves its counters zero again, which are its first
+ * GRINQH_KV4_COUNTER_BYTES); calls that share one must be ordered (same stream,
+ * and graphs that hold such calls replayed one after the other).  Its size grows with seqs up to 1024 sequences and
  * 2^15 pairs of a sequence and up to 16 query heads of one key/value head, and
  * is 0 beyond, where no sequence is shared between blocks: one workspace for
  * batches of many sizes is that of the largest batch within. */
+#define GRINQH_KV4_COUNTER_BYTES ((size_t)1 << 17)
 size_t grinqh_kv4_attention_workspace_bytes(int64_t seqs, int heads, int kv_heads, int head_dim, int64_t capacity);
 int grinqh_kv4_attention(const void* q, int64_t q_token, int64_t q_head, int64_t seqs, int heads, const void* cache,
                          int64_t pages, int kv_heads, int page_size, int head_dim, int group,
@@ -330,6 +332,11 @@ int grinqh_kv4_select(const void* q, int64_t q_token, int64_t q_head, int64_t se
                       int64_t pages, int kv_heads, int page_size, int head_dim, const int32_t* page_table,
                       int64_t table_stride, int table_width, const int32_t* lengths, int count, int32_t* selected,
                       int32_t* new_lengths, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The number of the graph capture that `stream` takes part in, 0 if it takes part
+ * in none.  No two captures of a process have the same, so that a caller can
+ * give each graph a workspace of its own.  No counterpart in the reference. */
+uint64_t grinqh_capture_id(void* stream);
 
 /* Benchmark instrumentation; no counterpart in the reference.  Arms a one-shot
  * timer: in the next grinqh_gemm_or_gemv / grinqh_gemv_batch_union /

@@ -740,7 +740,19 @@ int grinqh_expire_tile_waits(int on) {
   return before;
 }
 
+uint64_t grinqh_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(as_stream(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 // ---- attention
+
+static_assert(kKv4Counters * sizeof(uint32_t) == GRINQH_KV4_COUNTER_BYTES, "as the header says");
 
 size_t grinqh_kv4_record_bytes(int head_dim, int group) {
   return valid_head(head_dim, group) ? (size_t)kv4_record_bytes(head_dim, head_dim / group) : 0;

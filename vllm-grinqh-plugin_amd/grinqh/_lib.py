@@ -21,6 +21,7 @@ GRINQH_ERR_WORKSPACE = 3
 GRINQH_ERR_SCRATCH = 4
 NOALLOC_SCRATCH_BYTES = 64 << 20
 SIGMA_CHUNK_ROWS = 16
+KV4_COUNTER_BYTES = 1 << 17
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -80,6 +81,7 @@ SIGNATURES = {
                                  _vp, _vp, _i32, _vp, ctypes.c_size_t, _vp]),
     "grinqh_time_next_product": (_i32, [_vp, _vp]),
     "grinqh_expire_tile_waits": (_i32, [_i32]),
+    "grinqh_capture_id": (ctypes.c_uint64, [_vp]),
     "grinqh_product_kernel": (_i32, [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
                                      ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
 }

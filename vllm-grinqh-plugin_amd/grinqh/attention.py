@@ -18,6 +18,7 @@ attention to vLLM.
 """
 from __future__ import annotations
 
+import threading
 from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
@@ -33,6 +34,37 @@ GROUPS = (32, 64, 128, 256)
 # Counters and partial results of split sequences; the linears' workspaces have
 # counters of their own at the same place.
 _WORKSPACES = _Workspaces()
+
+
+class _GraphWorkspaces:
+    """Workspaces of captured calls, in the graph's own memory, so that graphs which were captured on one stream may be
+    replayed at the same time on several: one for all calls of a capture on a stream, which follow each other.  The
+    counters are cleared once in every replay, in front of the first call; every call leaves them zero.  Kept here until
+    the stream's next capture, as the memory must not be given to anything between two calls of a graph."""
+
+    def __init__(self):
+        self._bufs = {}  # (device, stream) -> (capture, buffer)
+        self._lock = threading.Lock()
+
+    def get(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+        key, capture = (device.index, stream), _lib.load_library().grinqh_capture_id(stream)
+        with self._lock:
+            before, ws = self._bufs.get(key, (0, None))
+            if before != capture or capture == 0 or ws.numel() < nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                ws[:_lib.KV4_COUNTER_BYTES].zero_()
+                self._bufs[key] = capture, ws
+            return ws
+
+
+_GRAPH_WORKSPACES = _GraphWorkspaces()
+
+
+def _workspace(device: torch.device, stream: int, nbytes: int) -> Optional[torch.Tensor]:
+    """The stream's workspace, or the graph's that is being captured; for the current device"""
+    if nbytes == 0:
+        return None
+    return (_GRAPH_WORKSPACES if torch.cuda.is_current_stream_capturing() else _WORKSPACES).get(device, stream, nbytes)
 
 
 def kv4_record_bytes(head_dim: int, group: Optional[int] = None) -> int:
@@ -135,8 +167,8 @@ def _scale(scale: Optional[float], head_dim: int) -> float:
 
 @lru_cache(maxsize=1024)
 def _workspace_bytes(seqs: int, heads: int, kv_heads: int, head_dim: int, capacity: int) -> int:
-    """Workspace of this batch and of every smaller one, so that a program which ran its largest batch can capture the
-    others: the library's sizes grow with the batch up to the largest that may share its sequences between blocks, and
+    """Workspace of this batch and of every smaller one, so that batches of changing size need no larger one: the
+    library's sizes grow with the batch up to the largest that may share its sequences between blocks, and
     are 0 beyond."""
     tiles = kv_heads * -(-(heads // kv_heads) // 16)
     seqs = min(seqs, _SHARED_SEQS, _SHARED_UNITS // tiles) if heads >= kv_heads else seqs
@@ -203,7 +235,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     with _lib.on_device(dev):
         stream = _stream(dev.index)
         nbytes = _workspace_bytes(seqs, heads, kv_heads, d, width * page)
-        ws = _WORKSPACES.get(dev, stream, nbytes) if nbytes else None
+        ws = _workspace(dev, stream, nbytes)
         at, room = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
         if table_head is None:
             _lib.check(_lib.load_library().grinqh_kv4_attention(
@@ -328,26 +360,13 @@ def kv4_chunk_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.
     nbytes = _chunk_workspace_bytes(tokens, seqs, heads, kv_heads, d, width * page)
     with _lib.on_device(dev):
         stream = _stream(dev.index)
-        ws = _chunk_workspace(dev, stream, nbytes) if nbytes else None
+        ws = _workspace(dev, stream, nbytes)
         _lib.check(_lib.load_library().grinqh_kv4_chunk_attention(
             q.data_ptr(), q_token, q_head, tokens, heads, cache.data_ptr(), pages, kv_heads, page, d, group,
             page_table.data_ptr(), table_stride, width, lengths.data_ptr(), ends.data_ptr(), seqs, _scale(scale, d),
             out.data_ptr(), dt, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
             "grinqh_kv4_chunk_attention")
     return out
-
-
-_COUNTER_BYTES = 1 << 17
-
-
-def _chunk_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """The stream's workspace; in a graph that is being captured one of its own, so that graphs replayed at the same
-    time on different streams do not meet in it (their counters are then cleared in every replay)"""
-    if not torch.cuda.is_current_stream_capturing():
-        return _WORKSPACES.get(device, stream, nbytes)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    ws[:_COUNTER_BYTES].zero_()
-    return ws
 
 
 @lru_cache(maxsize=1024)
