@@ -74,6 +74,13 @@ class Decoder:
         self.before, self.lengths, self.free_count = self.lengths, room.lengths, room.free_count
         return room
 
+    def all_have_room(self) -> bool:
+        """Whether every token so far found a page; waits for the GPU.  A server that may run out looks at this before it
+        hands out results, and makes the step again from ``before`` and its list of free pages when some have come free."""
+        pages = (self.lengths + self.page - 1) // self.page
+        place = torch.arange(self.max_pages, device="cuda")
+        return bool(((self.table >= 0) | (place >= pages.view(-1, 1))).all()) and int(pages.max()) <= self.max_pages
+
     def _rotate(self, x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
         angle = position.float().view(-1, 1, 1) * self.freq
         a, b = x.float().chunk(2, -1)
@@ -138,6 +145,7 @@ def main() -> None:
         torch.cuda.synchronize()
         t = (time.perf_counter() - start) / (steps // 2)
         what = f"{select} pages per head" if select else "all pages"
+        assert model.all_have_room()
         print(f"4 layers, batch {batch}, {length} tokens of context, {what}: {t * 1e3:.2f} ms a step (eager)")
 
 

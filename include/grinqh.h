@@ -282,7 +282,11 @@ int grinqh_kv4_attention_selected(const void* q, int64_t q_token, int64_t q_head
  * place) and its position in the sequence; rows behind the last sequence, places
  * behind the table and pages that are missing (-1 in the table, too) have slot -1.
  * new_lengths and new_free_count hold what is left; lengths, counts, free_pages and
- * free_count are not changed and must not overlap the results. */
+ * free_count are not changed and must not overlap the results.  Tokens without a
+ * page are counted in new_lengths, and later calls do not look for their pages: a
+ * slot of -1 in front of row ends[seqs] says that there were too few.  The same call
+ * again from the old lengths and list, with fewer tokens or more free pages behind
+ * that list, writes the same entries of the table anew. */
 int grinqh_kv4_append(int32_t* page_table, int64_t table_stride, int table_width, int page_size,
                       const int32_t* lengths, const int32_t* counts, int64_t seqs, const int32_t* free_pages,
                       int64_t free_size, const int32_t* free_count, int64_t tokens, int64_t* slots, int32_t* positions,

@@ -305,7 +305,10 @@ def kv4_append(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Te
     place; nothing else that is given changes.  ``tokens`` is the number of rows of the batch's buffers, the new tokens
     packed in front: rows behind the last sequence have slot -1, tokens that do not fit are not counted.  Where pages
     run out the table gets -1, and where it ends nothing: such tokens have slot -1 (``kv4_store`` skips them) and the
-    attention of their sequences is NaN."""
+    attention of their sequences is NaN.  They are counted in the lengths, and later calls do not look for their pages
+    again: a slot of -1 in front of row ``ends[-1]`` says so.  The call is then made again from the lengths and the list
+    that it was given, which it has not changed, with fewer tokens or when pages have been put behind that list; it writes
+    the same entries of the table anew."""
     dev = page_table.device
     if not page_table.is_cuda:
         raise ValueError(f"GRINQH: page_table must be on a HIP device (got {dev}); there is no CPU path")
