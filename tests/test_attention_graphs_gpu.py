@@ -125,3 +125,25 @@ def test_steps_over_selected_pages_on_two_streams():
         for a, b, out, want in zip(captured, eager, outs, wants):
             assert torch.equal(a.lengths, b.lengths) and torch.equal(a.table, b.table)
             assert torch.equal(out, want), turn
+
+
+def test_two_streams_of_one_capture():
+    """a graph whose calls run beside each other"""
+    from grinqh import attention as ga
+    rng = np.random.default_rng(6)
+    cache, table, lengths, _ = _paged(rng, [9000, 3000], 2, 128, 16, 64, "f16")
+    qs = [_randn(rng, 2, 8, 128) for _ in range(2)]
+    rows, ends = _randn(rng, 40, 8, 128), _i32([0, 3, 40])
+
+    def program(other):
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            outs = [ga.kv4_attention(qs[0], cache, table, lengths), ga.kv4_chunk_attention(rows, cache, table, lengths, ends)]
+        outs += [ga.kv4_attention(qs[1], cache, table, lengths), ga.kv4_chunk_attention(rows, cache, table, lengths, ends)]
+        here.wait_stream(other)
+        return outs
+
+    want = program(torch.cuda.Stream())
+    graph, out = _captured(lambda: program(torch.cuda.Stream()), torch.cuda.Stream())
+    _replayed([graph], [out], [want], lambda: program(torch.cuda.Stream()))
