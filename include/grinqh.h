@@ -299,7 +299,11 @@ int grinqh_kv4_append(int32_t* page_table, int64_t table_stride, int table_width
  * or behind the last give zeros; a length past the table makes the sequence's
  * results NaN, a page outside the cache those of the rows that see its tokens (and
  * perhaps others of the sequence).
- * Tokens that a row does not see have no effect on it.  At most 2^20 sequences;
+ * Tokens that a row does not see, and what the pages hold behind the last one, have
+ * no effect on it.  Which rows are beside a sequence decides how its work is split and
+ * which of two kernels does it, and so its roundings: keys, values and weights in fp16, or
+ * the cache's codes exactly and weights in fp16.  At most 2^20 sequences, whose offsets
+ * and lengths every block looks at (64 at a time);
  * the workspace (..._workspace_bytes for a capacity of table_width * page_size
  * tokens, 256-byte aligned) is zero-filled once before its first use, as that of
  * grinqh_kv4_attention, with which it can be one; calls that share it must be ordered. */
@@ -314,7 +318,8 @@ int grinqh_kv4_chunk_attention(const void* q, int64_t q_token, int64_t q_head, i
 /* The mean key of every page that tokens starts[s] .. lengths[s] - 1 of a sequence
  * lie in (tokens in front of starts[s] in the first one counted), in 8 bits.  The
  * summary is int8 [pages][kv_heads][head_dim + 16], 16-byte aligned: head_dim
- * codes, their fp32 step, 12 unused bytes.  With m the mean (exact sums in 64 bits)
+ * codes, their fp32 step, 12 unused bytes.  With m the mean (of sums in 64 bits, which
+ * are exact for pages of up to 4096 tokens; of more they are rounded, always alike)
  * and 2^E <= max |m| < 2^(E + 1): step = 2^(E - 6), code = round(m / step) within
  * +-127; NaN channels count as 0, a page of zeros has step 0.  Pages outside the cache
  * and tokens behind the table are passed over. */

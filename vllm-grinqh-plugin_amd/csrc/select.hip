@@ -8,7 +8,8 @@
 // heads' products codes(q).codes(m), times both steps: whole numbers below 2^22
 // times powers of two, so nothing is rounded and the selection does not depend on
 // the order of any sum.  The means are sums in 64 bits that are exact too: what a code
-// stands for is a multiple of 2^-24 below 2^17, and 4096 tokens of it fit 53 bits.
+// stands for is a multiple of 2^-24 below 2^17, and 4096 tokens of it fit 53 bits; longer
+// pages' sums are rounded, in the order of the lanes, which is always the same.
 //
 // All are bound by latency: of a page's records (summaries: 32 tokens' pages 4.7 us, 4
 // prompts of 2048 tokens 7.4 us, 0.8 TB/s), of the search for the last selected score.

@@ -344,7 +344,8 @@ def kv4_chunk_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.
     ``lengths[s]`` (int32) tokens of its pages ``page_table[s]`` (int32 ``[seqs, width]``).  Its last row sees all of
     them, the row before one fewer, and so on.  Rows that see none, in front of the first sequence or behind the last
     give zeros; a length past the table makes the sequence's rows NaN, a page outside the cache those that see it (and
-    perhaps others of the sequence).  ``scale`` defaults to head_dim ** -0.5."""
+    perhaps others of the sequence).  ``scale`` defaults to head_dim ** -0.5.  What is beside a sequence in the batch
+    may change its results by their roundings; the same call gives the same bits."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
     dev, dtype = cache.device, q.dtype
     dt = _dtype_code(dtype)
@@ -401,7 +402,8 @@ def kv4_summarize(cache: torch.Tensor, summary: torch.Tensor, page_table: torch.
                   lengths: torch.Tensor) -> None:
     """Bring ``summary`` up to date for every page that tokens ``starts[s] .. lengths[s] - 1`` of a sequence lie in
     (int32 ``[seqs]`` both: the lengths before and after ``kv4_append``; 0 and the lengths for all of their pages).
-    Called after ``kv4_store``.  Sequences that share a page must agree on how many of its tokens count."""
+    Called after ``kv4_store``.  Sequences that share a page must agree on how many of its tokens count.  Sums are exact
+    for pages of up to 4096 tokens."""
     pages, kv_heads, page, d, group = _cache_layout(cache)
     dev = cache.device
     if _summary_layout(summary) != (pages, kv_heads, d) or summary.device != dev:
@@ -424,7 +426,7 @@ def kv4_select(q: torch.Tensor, summary: torch.Tensor, page_table: torch.Tensor,
     sequence and key/value head whose mean keys promise the largest logits; the first page and the last are always
     among them.  Returns a page table per head, int32 ``[seqs, kv_heads, count]`` in the order of the sequence (-1 behind
     the last page), and how many tokens the selected pages hold, int32 ``[seqs]``: both as ``kv4_attention`` takes them.
-    Scores are exact, equal ones go to the page that comes first."""
+    Scores are exact sums of what the summaries hold, equal ones go to the page that comes first."""
     pages, kv_heads, d = _summary_layout(summary)
     dev, dtype = summary.device, q.dtype
     dt = _dtype_code(dtype)
